@@ -234,10 +234,12 @@ def _plain_distill(s):
 
 
 # ------------------------------------------------------------------------------------------------ this repository
+_PACKAGE = str(Path(__file__).resolve().parents[1] / "ai-compiler-framework_b200" / "python")
+
+
 def _aicf():
-    path = str(Path(__file__).resolve().parents[1] / "ai-compiler-framework_b200" / "python")
-    if path not in sys.path:
-        sys.path.insert(0, path)
+    if _PACKAGE not in sys.path:
+        sys.path.insert(0, _PACKAGE)
     import aicf_cuda
     return aicf_cuda
 
