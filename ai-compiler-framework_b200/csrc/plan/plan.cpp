@@ -53,6 +53,8 @@ bool kind_of(const std::string& name, OpKind* k) {
       {"reduce_max", OpKind::ReduceMax},  {"reduce_mean", OpKind::ReduceMean}, {"all_reduce", OpKind::AllReduce},
       {"cast", OpKind::Cast},             {"gemm_relu_bwd", OpKind::GemmReluBwd},
       {"dp_adam_step", OpKind::DpAdamStep},
+      {"quant_fp8", OpKind::QuantFp8},
+      {"distill_ce", OpKind::DistillCE},
   };
   auto it = kMap.find(name);
   if (it == kMap.end()) return false;

@@ -34,6 +34,7 @@ enum class OpKind : int {
   BatchNormBwd = 16, GemmEpilogue = 17,
   // additions of this backend
   Softmax = 18, SoftmaxCE = 19, ReduceMax = 20, ReduceMean = 21, AllReduce = 22, Cast = 23, GemmReluBwd = 24, DpAdamStep = 25,
+  QuantFp8 = 26, DistillCE = 27,
 };
 
 [[noreturn]] void raise_last(const char* what, int rc) {
@@ -50,7 +51,9 @@ int dtype_code_from_name(const std::string& n) {
       {"f32", 1}, {"float32", 1}, {"torch.float32", 1}, {"torch.float", 1},
       {"f16", 2}, {"float16", 2}, {"torch.float16", 2}, {"torch.half", 2},
       {"bf16", 3}, {"bfloat16", 3}, {"torch.bfloat16", 3},
-      {"i32", 4}, {"int32", 4}, {"torch.int32", 4}, {"torch.int", 4}};
+      {"i32", 4}, {"int32", 4}, {"torch.int32", 4}, {"torch.int", 4},
+      {"f8e4m3", 5}, {"float8_e4m3fn", 5}, {"torch.float8_e4m3fn", 5},
+      {"f8e5m2", 6}, {"float8_e5m2", 6}, {"torch.float8_e5m2", 6}};
   auto it = kByName.find(n);
   return it == kByName.end() ? 0 : it->second;
 }
@@ -65,7 +68,7 @@ int dtype_code(const py::handle& dtype) {
   if (it != cache->end()) return it->second;
   const std::string name = py::str(dtype);
   const int code = dtype_code_from_name(name);
-  if (code == 0) throw std::runtime_error("dtype must be float16/bfloat16/float32/int32. got: dtype=" + name);
+  if (code == 0) throw std::runtime_error("dtype must be float16/bfloat16/float32/int32/float8_e4m3fn/float8_e5m2. got: dtype=" + name);
   if (cache->size() < 64) {
     Py_INCREF(dtype.ptr());  // kept for the life of the process
     cache->emplace(dtype.ptr(), code);
@@ -158,6 +161,7 @@ PYBIND11_MODULE(_C, m) {
       .value("GemmEpilogue", OpKind::GemmEpilogue).value("Softmax", OpKind::Softmax).value("SoftmaxCE", OpKind::SoftmaxCE)
       .value("ReduceMax", OpKind::ReduceMax).value("ReduceMean", OpKind::ReduceMean).value("AllReduce", OpKind::AllReduce)
       .value("Cast", OpKind::Cast).value("GemmReluBwd", OpKind::GemmReluBwd).value("DpAdamStep", OpKind::DpAdamStep)
+      .value("QuantFp8", OpKind::QuantFp8).value("DistillCE", OpKind::DistillCE)
       .export_values();
 
   m.def("op_call", &op_call, py::arg("kind"), py::arg("inputs"), py::arg("outputs"), py::arg("schema_id") = 0,

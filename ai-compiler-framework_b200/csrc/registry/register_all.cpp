@@ -91,6 +91,22 @@ KernelVariant make_gemm_bias_relu_f16_tcgen05_out_f16_variant();
 KernelVariant make_gemm_relu_bwd_bf16_variant();
 KernelVariant make_gemm_relu_bwd_f16_variant();
 KernelVariant make_gemm_relu_bwd_f32_variant();
+// quant_fp8.cu
+KernelVariant make_quant_fp8_block128_variant();
+// gemm_fp8.cu
+KernelVariant make_gemm_fp8_block128_out_f32_variant();
+KernelVariant make_gemm_fp8_block128_out_bf16_variant();
+KernelVariant make_gemm_fp8_block128_out_f16_variant();
+KernelVariant make_gemm_bias_relu_fp8_block128_out_f32_variant();
+KernelVariant make_gemm_bias_relu_fp8_block128_out_bf16_variant();
+KernelVariant make_gemm_bias_relu_fp8_block128_out_f16_variant();
+KernelVariant make_gemm_relu_bwd_fp8_block128_out_f32_variant();
+KernelVariant make_gemm_relu_bwd_fp8_block128_out_bf16_variant();
+KernelVariant make_gemm_relu_bwd_fp8_block128_out_f16_variant();
+// distill_ce.cu
+KernelVariant make_distill_ce_f32_variant();
+KernelVariant make_distill_ce_bf16_variant();
+KernelVariant make_distill_ce_f16_variant();
 // allreduce.cpp
 KernelVariant make_all_reduce_nccl_f32_variant();
 // dp_adam.cu
@@ -192,6 +208,19 @@ extern "C" void aicf_cuda_register_all_kernels() {
       {K::GemmReluBwd, make_gemm_relu_bwd_f16_variant, 10, "gemm_relu_bwd_f16_tcgen05_out_f16_v0"},
       {K::GemmReluBwd, make_gemm_relu_bwd_f32_variant, 0, "gemm_relu_bwd_f32_v0"},
       {K::GemmReluBwd, make_gemm_relu_bwd_f32_3xtf32_variant, -20, "gemm_relu_bwd_f32_3xtf32_v0"},
+      {K::QuantFp8, make_quant_fp8_block128_variant, 0, "quant_fp8_block128_v0"},
+      {K::Gemm, make_gemm_fp8_block128_out_bf16_variant, 10, "gemm_fp8_block128_out_bf16_v0"},
+      {K::Gemm, make_gemm_fp8_block128_out_f16_variant, 10, "gemm_fp8_block128_out_f16_v0"},
+      {K::Gemm, make_gemm_fp8_block128_out_f32_variant, 10, "gemm_fp8_block128_out_f32_v0"},
+      {K::GemmEpilogue, make_gemm_bias_relu_fp8_block128_out_bf16_variant, 10, "gemm_bias_relu_fp8_block128_out_bf16_v0"},
+      {K::GemmEpilogue, make_gemm_bias_relu_fp8_block128_out_f16_variant, 10, "gemm_bias_relu_fp8_block128_out_f16_v0"},
+      {K::GemmEpilogue, make_gemm_bias_relu_fp8_block128_out_f32_variant, 10, "gemm_bias_relu_fp8_block128_out_f32_v0"},
+      {K::GemmReluBwd, make_gemm_relu_bwd_fp8_block128_out_bf16_variant, 5, "gemm_relu_bwd_fp8_block128_out_bf16_v0"},
+      {K::GemmReluBwd, make_gemm_relu_bwd_fp8_block128_out_f16_variant, 5, "gemm_relu_bwd_fp8_block128_out_f16_v0"},
+      {K::GemmReluBwd, make_gemm_relu_bwd_fp8_block128_out_f32_variant, 5, "gemm_relu_bwd_fp8_block128_out_f32_v0"},
+      {K::DistillCE, make_distill_ce_f32_variant, 0, "distill_ce_f32_v0"},
+      {K::DistillCE, make_distill_ce_bf16_variant, 0, "distill_ce_bf16_v0"},
+      {K::DistillCE, make_distill_ce_f16_variant, 0, "distill_ce_f16_v0"},
       {K::AllReduce, make_all_reduce_nccl_f32_variant, 0, "all_reduce_nccl_f32_v0"},
       {K::DpAdamStep, make_dp_adam_step_variant, 0, "dp_adam_step_f32_p2p_v0"},
   };

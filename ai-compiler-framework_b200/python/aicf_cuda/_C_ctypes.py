@@ -51,6 +51,8 @@ class OpKind(enum.IntEnum):
     Cast = 23
     GemmReluBwd = 24
     DpAdamStep = 25
+    QuantFp8 = 26
+    DistillCE = 27
 
 
 # pybind's export_values(): enumerators are also module attributes
@@ -62,6 +64,8 @@ _DTYPE_BY_NAME = {
     "f16": 2, "float16": 2, "torch.float16": 2, "torch.half": 2,
     "bf16": 3, "bfloat16": 3, "torch.bfloat16": 3,
     "i32": 4, "int32": 4, "torch.int32": 4, "torch.int": 4,
+    "f8e4m3": 5, "float8_e4m3fn": 5, "torch.float8_e4m3fn": 5,
+    "f8e5m2": 6, "float8_e5m2": 6, "torch.float8_e5m2": 6,
 }
 
 
@@ -69,7 +73,7 @@ def _dtype_code(t: Any) -> int:
     name = str(getattr(t, "dtype", None))
     code = _DTYPE_BY_NAME.get(name)
     if code is None:
-        raise RuntimeError(f"dtype must be float16/bfloat16/float32/int32. got: dtype={name}")
+        raise RuntimeError(f"dtype must be float16/bfloat16/float32/int32/float8_e4m3fn/float8_e5m2. got: dtype={name}")
     return code
 
 

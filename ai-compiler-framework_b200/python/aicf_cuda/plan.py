@@ -30,6 +30,7 @@ SCHEMA_LAYERNORM = 0x50454E4C  # 'LNEP'
 
 SCHEMA_ALL_REDUCE = 0x44455241
 SCHEMA_DP_ADAM = 0x44415044
+SCHEMA_DISTILL = 0x4C545344  # 'DSTL'
 # What the reference's Python executor sends for gemm_epilogue (exec.py:215-217); the reference's C++
 # does not know this tag and silently applies its defaults.
 SCHEMA_GEPI_AS_SENT_BY_REFERENCE_EXECUTOR = int.from_bytes(b"GEPI", "little")
@@ -85,6 +86,10 @@ def pack_attrs(op: str, attrs: Optional[Dict[str, Any]]) -> Tuple[int, bytes]:
         return SCHEMA_BIAS_ADD, struct.pack("<q", int(a["axis"]))
     if op == "softmax_ce" and "scale" in a:
         return SCHEMA_SOFTMAX_CE, struct.pack("<f", float(a["scale"]))
+    if op == "distill_ce" and a:
+        if "scale" not in a:
+            raise ValueError("distill_ce: attrs need 'scale' (1 / batch for the mean over the rows)")
+        return SCHEMA_DISTILL, struct.pack("<fff", float(a["scale"]), float(a.get("temperature", 1.0)), float(a.get("alpha", 0.0)))
     if op == "layernorm_fwd" and "eps" in a:
         return SCHEMA_LAYERNORM, struct.pack("<f", float(a["eps"]))
     if op == "all_reduce":

@@ -33,6 +33,7 @@ constexpr uint32_t kBatchNorm = 0x50454E42u;
 // additions
 constexpr uint32_t kSoftmaxCE = 0x45434D53u;     // 'SMCE' LE: <f> scale
 constexpr uint32_t kAllReduce = 0x44455241u;     // 'ARED' LE: <i> bucket id
+constexpr uint32_t kDistill = 0x4C545344u;       // 'DSTL' LE: <fff> scale, temperature, alpha
 }  // namespace schema
 
 }  // namespace aicf::cuda

@@ -36,7 +36,10 @@ enum class OpKind : int {
 
   DpAdamStep = 25,  // data-parallel Adam fused with its gradient exchange over peer memory
 
-  _Count = 26,
+  QuantFp8 = 26,    // matrix -> 8-bit floating point with one fp32 scale per block of 128 (rows, columns, both, tiles)
+  DistillCE = 27,   // distillation from a teacher's top logits (optionally mixed with labels): loss rows, gradient
+
+  _Count = 28,
   // Number of kinds the reference defines; ids below this resolve exactly as there.
   _ReferenceCount = 18
 };
@@ -71,6 +74,8 @@ inline const char* op_kind_name(OpKind k) {
     case OpKind::Cast: return "cast";
     case OpKind::GemmReluBwd: return "gemm_relu_bwd";
     case OpKind::DpAdamStep: return "dp_adam_step";
+    case OpKind::QuantFp8: return "quant_fp8";
+    case OpKind::DistillCE: return "distill_ce";
     default: return "unknown";
   }
 }

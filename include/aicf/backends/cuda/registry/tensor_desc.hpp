@@ -15,6 +15,9 @@ enum class DType : uint8_t {
   kF16 = 2,
   kBF16 = 3,
   kI32 = 4,
+  // additions of this backend: 8-bit floating point, values of a block-scaled matrix
+  kF8E4M3 = 5,  // 4 exponent bits, 3 mantissa bits, largest value 448, no infinity
+  kF8E5M2 = 6,  // 5 exponent bits, 2 mantissa bits, largest value 57344
   // spellings the reference also accepts
   Unknown = kUnknown,
   F32 = kF32,
@@ -28,11 +31,12 @@ constexpr bool dtype_is_float(DType t) {
   return t == DType::kF32 || t == DType::kF16 || t == DType::kBF16;
 }
 constexpr bool dtype_is_int(DType t) { return t == DType::kI32; }
+constexpr bool dtype_is_fp8(DType t) { return t == DType::kF8E4M3 || t == DType::kF8E5M2; }
 constexpr bool dtype_is_supported(DType t) {
-  return dtype_is_float(t) || dtype_is_int(t) || t == DType::kUnknown;
+  return dtype_is_float(t) || dtype_is_int(t) || dtype_is_fp8(t) || t == DType::kUnknown;
 }
 constexpr int32_t dtype_bits(DType t) {
-  return (t == DType::kF32 || t == DType::kI32) ? 32 : (t == DType::kF16 || t == DType::kBF16) ? 16 : 0;
+  return (t == DType::kF32 || t == DType::kI32) ? 32 : (t == DType::kF16 || t == DType::kBF16) ? 16 : dtype_is_fp8(t) ? 8 : 0;
 }
 constexpr int32_t dtype_size_bytes(DType t) { return dtype_bits(t) / 8; }
 constexpr const char* dtype_name(DType t) {
@@ -41,6 +45,8 @@ constexpr const char* dtype_name(DType t) {
        : t == DType::kF16     ? "f16"
        : t == DType::kBF16    ? "bf16"
        : t == DType::kI32     ? "i32"
+       : t == DType::kF8E4M3  ? "f8e4m3"
+       : t == DType::kF8E5M2  ? "f8e5m2"
                               : "invalid";
 }
 // Accumulation type used by contractions and reductions.

@@ -23,7 +23,8 @@ extern "C" {
 /* ---- handle types ---------------------------------------------------------------------------
  * Bit-compatible with aicf::cuda::TensorDesc (include/aicf/backends/cuda/registry/tensor_desc.hpp:88-104,
  * sizeof 96) and aicf::cuda::AttrBlob (attr_blob.hpp:13-17, sizeof 16). */
-enum { AICF_DTYPE_UNKNOWN = 0, AICF_DTYPE_F32 = 1, AICF_DTYPE_F16 = 2, AICF_DTYPE_BF16 = 3, AICF_DTYPE_I32 = 4 };
+enum { AICF_DTYPE_UNKNOWN = 0, AICF_DTYPE_F32 = 1, AICF_DTYPE_F16 = 2, AICF_DTYPE_BF16 = 3, AICF_DTYPE_I32 = 4,
+       AICF_DTYPE_F8E4M3 = 5, AICF_DTYPE_F8E5M2 = 6 /* values of a block-scaled matrix: quant_fp8, *_fp8_block128_* */ };
 enum { AICF_OK = 0, AICF_INVALID_ARGUMENT = 1, AICF_NOT_IMPLEMENTED = 2, AICF_INTERNAL = 3 };
 
 typedef struct aicf_tensor_desc {

@@ -14,7 +14,8 @@ import numpy as np
 from . import ops as O
 
 _ROUND = {"f32": lambda a: np.asarray(a, np.float32), "bf16": O.bf16_round, "f16": O.f16_round,
-          "i32": lambda a: np.asarray(a, np.int32)}
+          "i32": lambda a: np.asarray(a, np.int32),
+          "f8e4m3": lambda a: O.fp8_round(a, "f8e4m3"), "f8e5m2": lambda a: O.fp8_round(a, "f8e5m2")}
 
 
 def _relu_flag(attrs: Dict[str, Any]) -> bool:
@@ -41,7 +42,27 @@ def run_lowered(lowered: Sequence[Dict[str, Any]], env: Dict[int, np.ndarray], d
         a = dict(it.get("attrs") or {})
         i = [env[v] for v in it["inputs"]]
         o = it["outputs"]
-        if op == "gemm":
+        if op in ("gemm", "gemm_epilogue", "gemm_relu_bwd") and dtypes[it["inputs"][0]].startswith("f8"):
+            c = O.gemm_fp8(i[0], i[1], i[-2], i[-1], a.get("transA", False), a.get("transB", False), dt)
+            if op == "gemm_epilogue":
+                c = c + np.asarray(i[2], dt)[None, :]
+                c = np.maximum(c, 0) if _relu_flag(a) else c
+            elif op == "gemm_relu_bwd":
+                c = O.relu_bwd(c, i[2], dt)
+            store(o[0], c)
+        elif op == "quant_fp8":
+            M, N = np.shape(i[0])
+            for q, s in zip(o[0::2], o[1::2]):
+                rows, cols = np.shape(env[s])[0] == M, np.shape(env[s])[1] == N
+                v, sc = O.quant_fp8(i[0], "rows" if rows else "cols" if cols else "tiles", dtypes[q])
+                store(q, v), store(s, sc)
+        elif op == "distill_ce":
+            d, loss = O.distill_ce(i[0], i[1], i[2], i[3] if len(i) > 3 else None, a.get("scale"), a.get("temperature", 1.0),
+                                   a.get("alpha", 0.0), dt)
+            store(o[-1], loss)
+            if len(o) > 1:
+                store(o[0], d)
+        elif op == "gemm":
             store(o[0], O.gemm(i[0], i[1], a.get("transA", False), a.get("transB", False), dt))
         elif op == "gemm_epilogue":
             store(o[0], O.gemm_epilogue(i[0], i[1], i[2], a.get("transA", False), a.get("transB", False), _relu_flag(a), dt))

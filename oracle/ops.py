@@ -7,7 +7,8 @@ import numpy as np
 
 __all__ = ["bf16_round", "f16_round", "gemm", "gemm_epilogue", "gemm_relu_bwd", "bias_add", "relu", "relu_bwd", "copy", "grad_zero",
            "mse_grad", "reduce_sum_columns", "reduce_lastaxis", "adam_step_v0", "adam_step_fused", "step_inc",
-           "bias_corr", "sgd_step", "add", "softmax", "softmax_ce", "cast", "layernorm_fwd", "layernorm_bwd"]
+           "bias_corr", "sgd_step", "add", "softmax", "softmax_ce", "cast", "layernorm_fwd", "layernorm_bwd",
+           "fp8_round", "quant_fp8", "dequant_fp8", "gemm_fp8", "distill_ce"]
 
 
 def bf16_round(x: np.ndarray) -> np.ndarray:
@@ -209,3 +210,83 @@ def layernorm_bwd(X, dY, gamma, mean, rstd, dt=np.float64):
         return dx, None, None
     lead = tuple(range(x.ndim - 1))
     return dx, (dy * xhat).sum(axis=lead), dy.sum(axis=lead)
+
+
+# ---- block-scaled 8-bit matrices and distillation (not in the reference) -----------------------------------------
+FP8_TOP = {"f8e4m3": 448.0, "f8e5m2": 57344.0}
+
+
+def fp8_round(x, fmt):
+    """Nearest value of the 8-bit format, ties to even, saturating; by arithmetic on the exponent, not by a table."""
+    x = np.asarray(x, np.float64)
+    mant, low = (3, -6) if fmt == "f8e4m3" else (2, -14)
+    a = np.minimum(np.abs(x), FP8_TOP[fmt])
+    e = np.maximum(np.frexp(np.where(a > 0, a, 1.0))[1] - 1, low)
+    step = np.ldexp(1.0, e - mant)
+    return np.where(np.isnan(x), np.nan, np.copysign(np.minimum(np.rint(a / step) * step, FP8_TOP[fmt]), x)).astype(np.float32)
+
+
+def _spread(s, shape):
+    """A scale matrix repeated to `shape`: each dimension is either whole or divided by 128."""
+    s = np.asarray(s)
+    for d in (0, 1):
+        if s.shape[d] != shape[d]:
+            s = np.take(s, np.arange(shape[d]) // 128, axis=d)
+    return s
+
+
+def quant_fp8(X, form, fmt):
+    """(q, s): per block ('rows' 1x128, 'cols' 128x1, 'tiles' 128x128) amax = max(max|x|, 2^-100), s = amax / F,
+    q = round(x * (F / amax)); both quotients and the product rounded to fp32 whatever the type of X."""
+    x = np.asarray(X, np.float32)
+    M, N = x.shape
+    by, bx = (128 if form in ("cols", "tiles") else 1), (128 if form in ("rows", "tiles") else 1)
+    mb, nb = -(-M // by), -(-N // bx)
+    padded = np.zeros((mb * by, nb * bx), np.float32)
+    padded[:M, :N] = x
+    with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
+        amax = np.maximum(np.abs(padded.reshape(mb, by, nb, bx)).max(axis=(1, 3)), np.float32(2.0 ** -100))
+        top = np.float32(FP8_TOP[fmt])
+        inv = (top / amax).astype(np.float32)
+        return fp8_round(x * _spread(inv, x.shape), fmt), (amax / top).astype(np.float32)
+
+
+def dequant_fp8(q, s, dt=np.float64):
+    return np.asarray(q, dt) * _spread(np.asarray(s, dt), np.shape(q))
+
+
+def gemm_fp8(A, B, SA, SB, transA=False, transB=False, dt=np.float64):
+    """op(A * SA) @ op(B * SB): scales spread over the stored operands."""
+    return gemm(dequant_fp8(A, SA, dt), dequant_fp8(B, SB, dt), transA, transB, dt)
+
+
+def distill_ce(logits, ids, teacher, labels=None, scale=None, temperature=1.0, alpha=0.0, dt=np.float64):
+    """(dlogits, loss_row): (1-alpha) T^2 KL(softmax(teacher / T) || softmax(z / T)) over the entries whose id lies in
+    [0, C), plus alpha times the cross-entropy of the label. A row without entries, or whose entries all are -inf, has no
+    first term; a row whose label lies outside [0, C) no second."""
+    z, t = np.asarray(logits, dt), np.asarray(teacher, dt)
+    ids = np.asarray(ids, np.int64)
+    B, Cn = z.shape
+    s = dt(1.0 / B) if scale is None else dt(scale)
+    T, al = dt(temperature), dt(alpha)
+    grad, loss = np.zeros((B, Cn), dt), np.zeros((B,), dt)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        for r in range(B):
+            ok = (ids[r] >= 0) & (ids[r] < Cn)
+            if ok.any() and not np.all(t[r][ok] == -np.inf):
+                zt, tt, cols = z[r] / T, t[r][ok] / T, ids[r][ok]
+                logq = zt - zt.max() - np.log(np.exp(zt - zt.max()).sum())
+                logp = tt - tt.max() - np.log(np.exp(tt - tt.max()).sum())
+                p = np.exp(logp)
+                loss[r] += (1 - al) * T * T * np.where(p == 0, 0, p * (logp - logq[cols])).sum()
+                g = np.exp(logq)
+                np.subtract.at(g, cols, p)
+                grad[r] += (1 - al) * T * g
+            lab = -1 if labels is None or al == 0 else int(labels[r])
+            if 0 <= lab < Cn:
+                log1 = z[r] - z[r].max() - np.log(np.exp(z[r] - z[r].max()).sum())
+                loss[r] -= al * log1[lab]
+                g = np.exp(log1)
+                g[lab] -= 1
+                grad[r] += al * g
+    return grad * s, loss
