@@ -11,6 +11,7 @@
 
 namespace aicf::cuda {
 int gemm_tcgen05_status(bool clear);
+int gemm_fp8_status(bool clear);
 int row_pipeline_status(bool clear);
 int layernorm_pipeline_status(bool clear);
 int adam_pipeline_status(bool clear);
@@ -242,12 +243,15 @@ int aicf_b200_gemm_reload_tuning(void) {
   aicf::cuda::gemm_reload_env_overrides();
   return AICF_OK;
 }
-int aicf_b200_gemm_status(int clear) { return aicf::cuda::gemm_tcgen05_status(clear != 0); }
+int aicf_b200_gemm_status(int clear) {
+  const int g = aicf::cuda::gemm_tcgen05_status(clear != 0), f = aicf::cuda::gemm_fp8_status(clear != 0);
+  return g != 0 ? g : f;
+}
 int aicf_b200_gemm_timeline(int enable, uint64_t* out16) {
   return aicf::cuda::gemm_tcgen05_timeline(enable, reinterpret_cast<unsigned long long*>(out16)) == 0 ? AICF_OK : AICF_INTERNAL;
 }
 int aicf_b200_wait_status(int clear) {
-  const int g = aicf::cuda::gemm_tcgen05_status(clear != 0);
+  const int g = aicf_b200_gemm_status(clear);
   const int rs = aicf::cuda::row_pipeline_status(clear != 0);
   const int rl = aicf::cuda::layernorm_pipeline_status(clear != 0);
   const int ra = aicf::cuda::adam_pipeline_status(clear != 0);

@@ -8,11 +8,23 @@
 // by 1 or by 128, which is what quant_fp8 writes (rows, columns or tiles). With K cut into blocks of 128,
 //
 //   C[m,n] = epilogue( sum over blocks kb of SA[m,kb] * SB[kb,n] * sum over k in kb of A[m,k] * B[k,n] )
-#include <cuda_fp8.h>
+//
+// The inner sums are tcgen05.mma.kind::f8f6f4 products (one k block = 128 bytes = one swizzle row = four MMAs of K = 32),
+// each accumulated from zero in a tensor-memory buffer of its own; the outer sum is held in fp32 registers by the eight
+// epilogue warps, which read a buffer back, scale it and add it while the next block is being multiplied. Roles, ring,
+// bounded waits and the CTA pair are those of the 16-bit kernel (gemm_tcgen05.cu): warp 0 TMA producer, warp 1 MMA issuer.
+// An operand contiguous along M / N instead of K is described to the MMA as MN-major, so no transposed copy is made.
+// Operands that TMA cannot address (rows not 16-byte aligned, or neither stride one) are first copied to aligned rows in
+// the workspace by repitch_kernel.
+#include <cstdlib>
+#include <type_traits>
 
 #include "gemm_common.cuh"
+#include "sm100_tcgen05.cuh"
 
 namespace aicf::cuda {
+
+using namespace sm100;
 
 namespace {
 
@@ -72,21 +84,94 @@ bool check(DType c_dtype, Epi epi, const TensorDesc* in, int ni, const TensorDes
   return true;
 }
 
+constexpr int kTileM = 128;        // rows of C per CTA
+constexpr int kTileK = 128;        // bytes of K per stage: one scale block, one 128-byte swizzle row
+constexpr int kUmmaK = 32;         // k extent of one kind::f8f6f4 MMA
+constexpr int kChunkBytes = kTileK * 128;   // MN-major operands: 128 k rows of 128 bytes
+constexpr int kRingBytes = 192 * 1024;
+constexpr int kEpiWarps = 8;
+constexpr int kFirstEpiWarp = 4;   // warps 2 and 3 have no work: they complete the first warpgroup
+constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
+// The 256-column tile holds 128 fp32 sums per epilogue thread. 384 threads are launched with 168 registers each; the first
+// warpgroup gives up 128 of its own and the two epilogue warpgroups take 64 more: 128 * 40 + 256 * 232 = 384 * 168.
+constexpr int kRegsLaunch = 168, kRegsRoles = 40, kRegsEpi = 232;
+static_assert(128 * kRegsRoles + 32 * kEpiWarps * kRegsEpi <= kThreads * kRegsLaunch, "the warpgroups' shares come out of the block's registers");
+constexpr int kGroupM = 16;        // tile rasterisation: 16 row tiles share their column tiles in L2
+constexpr unsigned long long kWaitBudgetNs = 1000000000ull;
+
+__device__ int g_fp8_status = 0;   // 0 ok; otherwise (role << 8) | reason of the first CTA that gave up
+
 struct Fp8Params {
-  const uint8_t *A, *B;
-  int64_t ars, acs, brs, bcs;
-  int a_e5m2, b_e5m2;
-  ScaleView sa, sb;
   void* C;
-  int64_t ldc;
-  int c_dtype;
   const void* bias;
-  int64_t bias_stride;
-  int bias_dtype, relu;
-  const void* mask;
-  int64_t mask_ld;
+  const void* mask;      // ReLU-backward mask, dtype of C
+  int64_t ldc, mask_ld, bias_stride;
+  ScaleView sa, sb;
   int M, N, K;
+  int c_dtype, bias_dtype;  // DType values, 0 = no bias
+  int relu;
+  int c_vec, mask_vec;   // rows of C (of the mask) allow 32-byte stores (16-byte loads)
+  int a_mn_major, b_mn_major;
+  uint32_t idesc;
+  int splits;            // CTAs of a cluster that share a tile, each with a range of k blocks (single-CTA kernel)
 };
+
+// Tile shapes. kCg CTAs work on one tile of kCg * 128 rows and kTn columns; each holds 128 rows of A and kTn / kCg columns of
+// B per stage, and a 128 x kTn accumulator.
+template <int kCg, int kTn> struct Cfg {
+  static constexpr int kBCols = kTn / kCg;
+  static constexpr int kABytes = kTileM * kTileK;
+  static constexpr int kStageBytes = kABytes + kBCols * kTileK;
+  static constexpr int kStages = kRingBytes / kStageBytes;
+  static constexpr int kBufs = kTn == 256 ? 2 : 4;          // accumulator buffers in tensor memory
+  static constexpr int kTmem = kBufs * kTn;
+  static constexpr int kCols = kTn / 2;                     // columns per epilogue warp
+  static constexpr size_t kStripBytes = size_t(kEpiWarps) * 2 * kCols * sizeof(float);
+  static constexpr size_t kSmem = 1024 + kRingBytes + 256 + kStripBytes;
+  static_assert(16 * kStages + 16 * kBufs + 8 <= 256, "barriers fit their 256 bytes");
+};
+
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
+  return mbar_wait_or_abort(bar, parity, abort_flag, &g_fp8_status, who, kWaitBudgetNs);
+}
+template <int kCg>
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (kCg == 1)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Shared-memory matrix descriptor, 128-byte swizzle, for 8-bit elements.
+//   K-major : rows of 128 B (128 elements of K); 1024 B between 8-row groups
+//   MN-major: 128 k rows of 128 B (128 elements of M / N) per chunk; 1024 B between 8-k groups, kChunkBytes between chunks
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, int mn_major) {
+  const uint64_t lbo = mn_major ? (kChunkBytes >> 4) : 1;
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (lbo << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Packed fp32 pairs: Blackwell's FMA pipe takes two per instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
   if (dtype == static_cast<int>(DType::kF32)) return static_cast<const float*>(p)[i];
@@ -98,72 +183,585 @@ __device__ __forceinline__ void store_from_f32(void* p, int64_t i, int dtype, fl
   else if (dtype == static_cast<int>(DType::kBF16)) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
-__device__ __forceinline__ float fp8_value(uint8_t b, int e5m2) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, e5m2 ? __NV_E5M2 : __NV_E4M3)));
+// 32 bytes = one whole DRAM sector per store
+__device__ __forceinline__ void st_sector(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
-// 64 x 64 outputs per block, 4 x 4 per thread, operands converted while they are staged; any strides.
-__global__ void __launch_bounds__(256) gemm_fp8_tile_kernel(const Fp8Params p, int tiles_n) {
-  __shared__ float As[16][64 + 1], Bs[16][64 + 1];
-  const int m0 = static_cast<int>(blockIdx.x / tiles_n) * 64, n0 = static_cast<int>(blockIdx.x % tiles_n) * 64;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {}, part[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += 16) {
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      const int r = i / 16, c = i % 16;
-      const int64_t m = m0 + r, n = n0 + r, k = k0 + c;
-      As[c][r] = m < p.M && k < p.K ? fp8_value(p.A[m * p.ars + k * p.acs], p.a_e5m2) : 0.0f;
-      Bs[c][r] = n < p.N && k < p.K ? fp8_value(p.B[k * p.brs + n * p.bcs], p.b_e5m2) : 0.0f;
-    }
-    __syncthreads();
-    for (int k = 0; k < 16; ++k)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) part[i][j] = fmaf(As[k][ty + 16 * i], Bs[k][tx + 16 * j], part[i][j]);
-    __syncthreads();
-    if ((k0 + 16) % kScaleBlk == 0 || k0 + 16 >= p.K) {
-      const int64_t kb = k0 / kScaleBlk;
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-          const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-          if (m < p.M && n < p.N)
-            // one factor after the other: the product of the scales may leave fp32 where the result does not
-            acc[i][j] += part[i][j] * p.sb.data[(n / p.sb.per) * p.sb.smn + kb * p.sb.sk] * p.sa.data[(m / p.sa.per) * p.sa.smn + kb * p.sa.sk];
-          part[i][j] = 0.0f;
+// 32 consecutive columns of one row of C: bias (from shared memory) and ReLU, or the ReLU-backward mask; convert; store.
+__device__ __forceinline__ void finish32(const Fp8Params& p, int row, int col0, float (&v)[32], const float* bias) {
+  if (p.bias_dtype != 0) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += bias[j];
+  }
+  if (p.relu) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];  // a NaN stays one
+  }
+  if (row >= p.M) return;
+  const bool whole = col0 + 32 <= p.N;
+  const bool f32 = p.c_dtype == static_cast<int>(DType::kF32), bf16 = p.c_dtype == static_cast<int>(DType::kBF16);
+  if (p.mask) {
+    const int64_t moff = static_cast<int64_t>(row) * p.mask_ld + col0;
+    if (whole && p.mask_vec && !f32) {
+      const uint4* ms = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.mask) + moff);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint4 y = __ldcs(ms + q);
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float lo, hi;
+          if (bf16) {
+            lo = __uint_as_float(w[e] << 16), hi = __uint_as_float(w[e] & 0xFFFF0000u);
+          } else {
+            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+            lo = t.x, hi = t.y;
+          }
+          if (!(lo > 0.0f)) v[8 * q + 2 * e] = 0.0f;
+          if (!(hi > 0.0f)) v[8 * q + 2 * e + 1] = 0.0f;
         }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col0 + j < p.N && !(load_as_f32(p.mask, moff + j, p.c_dtype) > 0.0f)) v[j] = 0.0f;
     }
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m >= p.M || n >= p.N) continue;
-      float v = acc[i][j];
-      if (p.bias) v += load_as_f32(p.bias, n * p.bias_stride, p.bias_dtype);
-      if (p.relu) v = fmaxf(v, 0.0f);
-      if (p.mask && !(load_as_f32(p.mask, m * p.mask_ld + n, p.c_dtype) > 0.0f)) v = 0.0f;
-      store_from_f32(p.C, m * p.ldc + n, p.c_dtype, v);
+  const int64_t off = static_cast<int64_t>(row) * p.ldc + col0;
+  if (f32) {
+    float* dst = static_cast<float*>(p.C) + off;
+    if (whole && p.c_vec) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(v[8 * q + e]);
+        st_sector(dst + 8 * q, w);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col0 + j < p.N) dst[j] = v[j];
     }
+    return;
+  }
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    if (bf16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  uint16_t* dst = static_cast<uint16_t*>(p.C) + off;
+  if (whole && p.c_vec) {
+    st_sector(dst, w);
+    st_sector(dst + 16, w + 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < p.N) dst[j] = static_cast<uint16_t>((j & 1) ? (w[j >> 1] >> 16) : (w[j >> 1] & 0xFFFFu));
+  }
 }
 
-Status run(const Fp8Problem& q, void*, size_t, cudaStream_t stream) {
+__device__ __forceinline__ void tile_of(int item, int tiles_m, int tiles_n, int group, int* tm, int* tn) {
+  const int per_group = group * tiles_n;
+  const int g = item / per_group;
+  const int first = g * group;
+  const int rows = min(group, tiles_m - first);
+  const int in_group = item - g * per_group;
+  *tm = first + in_group % rows;
+  *tn = in_group / rows;
+}
+
+// kVecB: the columns of B have a scale each (per = 1); otherwise 128 columns share one.
+template <int kCg, int kTn, bool kVecB>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const Fp8Params p) {
+  using F = Cfg<kCg, kTn>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_addr(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;  // 128B swizzle atoms repeat every 1024 B
+  uint8_t* base_ptr = smem_raw + (base - raw);
+  const uint32_t bar_full = base + kRingBytes, bar_empty = bar_full + 8 * F::kStages, bar_acc_full = bar_empty + 8 * F::kStages,
+                 bar_acc_empty = bar_acc_full + 8 * F::kBufs;
+  uint8_t* misc = base_ptr + kRingBytes + 16 * F::kStages + 16 * F::kBufs;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(misc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kCg == 2 || p.splits > 1 ? cluster_ctarank() : 0;
+  const bool leader = kCg == 1 || rank == 0;
+  const int splits = kCg == 1 ? p.splits : 1;
+  // work items: tiles, taken round-robin by clusters; CTA `split` of a split cluster takes a range of the tile's k blocks
+  const int first_item = kCg == 2 || splits > 1 ? static_cast<int>(cluster_id_x()) : static_cast<int>(blockIdx.x);
+  const int item_step = kCg == 2 || splits > 1 ? static_cast<int>(cluster_count_x()) : static_cast<int>(gridDim.x);
+  const int split = splits > 1 ? static_cast<int>(rank) : 0;
+  const int tiles_m = (p.M + kCg * kTileM - 1) / (kCg * kTileM), tiles_n = (p.N + kTn - 1) / kTn;
+  const int items = tiles_m * tiles_n;
+  const int k_blocks = (p.K + kTileK - 1) / kTileK;
+  const int kb_per = (k_blocks + splits - 1) / splits;
+  const int kb_lo = split * kb_per, kb_hi = min(kb_lo + kb_per, k_blocks);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < F::kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int b = 0; b < F::kBufs; ++b) {
+      mbar_init(bar_acc_full + 8 * b, 1);
+      mbar_init(bar_acc_empty + 8 * b, kCg * kEpiWarps);
+    }
+    *abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 1) {
+    const uint32_t slot = smem_addr(const_cast<uint32_t*>(tmem_slot));
+    if constexpr (kCg == 1) tmem_alloc(slot, F::kTmem);
+    else tmem_alloc_pair(slot, F::kTmem);
+  }
+  tc_fence_before();
+  if constexpr (kCg == 2) cluster_sync_all();  // both CTAs' barriers exist before anybody signals across the pair
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp < kFirstEpiWarp) {
+  if constexpr (kTn == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRoles));
+  if (warp == 0) {
+    // ---------------- TMA producer: in a pair each CTA loads its own halves, completion lands on the leader's barrier
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool alive = true;
+      for (int item = first_item; item < items && alive; item += item_step) {
+        int tm, tn;
+        tile_of(item, tiles_m, tiles_n, max(kGroupM / kCg, 1), &tm, &tn);
+        const int m0 = (tm * kCg + (kCg == 2 ? static_cast<int>(rank) : 0)) * kTileM;
+        const int n0 = tn * kTn + (kCg == 2 ? static_cast<int>(rank) * F::kBCols : 0);
+        for (int kb = kb_lo; kb < kb_hi; ++kb) {
+          if (!wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, 1)) { alive = false; break; }
+          const uint32_t sa = base + stage * F::kStageBytes, sb = sa + F::kABytes;
+          const int k0 = kb * kTileK;
+          const int ax = p.a_mn_major ? m0 : k0, ay = p.a_mn_major ? k0 : m0;
+          const int bx = p.b_mn_major ? n0 : k0, by = p.b_mn_major ? k0 : n0;
+          if constexpr (kCg == 2) {
+            const uint32_t full = map_to_cta(bar_full + 8 * stage, 0);
+            if (leader) mbar_expect_tx(bar_full + 8 * stage, 2 * F::kStageBytes);
+            tma_load_2d_pair(sa, &tmap_a, ax, ay, full);
+            tma_load_2d_pair(sb, &tmap_b, bx, by, full);
+          } else {
+            const uint32_t full = bar_full + 8 * stage;
+            mbar_expect_tx(full, F::kStageBytes);
+            tma_load_2d(sa, &tmap_a, ax, ay, full);
+            tma_load_2d(sb, &tmap_b, bx, by, full);
+            if (kTn == 256 && p.b_mn_major) tma_load_2d(sb + kChunkBytes, &tmap_b, bx + 128, by, full);
+          }
+          if (++stage == F::kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer: one lane, in a pair the leader's
+    if (leader && lane == 0) {
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      bool alive = true;
+      const uint32_t a_step = p.a_mn_major ? (kUmmaK * 128) >> 4 : kUmmaK >> 4;  // descriptor units of 16 B
+      const uint32_t b_step = p.b_mn_major ? (kUmmaK * 128) >> 4 : kUmmaK >> 4;
+      for (int item = first_item; item < items && alive; item += item_step) {
+        for (int kb = kb_lo; kb < kb_hi; ++kb) {
+          if (!wait(bar_acc_empty + 8 * buf, buf_phase ^ 1u, abort_flag, 2)) { alive = false; break; }
+          if (!wait(bar_full + 8 * stage, phase, abort_flag, 3)) { alive = false; break; }
+          tc_fence_after();
+          const uint32_t sa = base + stage * F::kStageBytes, sb = sa + F::kABytes;
+          const uint64_t adesc = smem_desc(sa, p.a_mn_major), bdesc = smem_desc(sb, p.b_mn_major);
+#pragma unroll
+          for (int k = 0; k < kTileK / kUmmaK; ++k)
+            umma_f8<kCg>(tmem_base + buf * kTn, adesc + k * a_step, bdesc + k * b_step, p.idesc, k != 0 ? 1u : 0u);
+          if constexpr (kCg == 2) {
+            umma_commit_pair(bar_empty + 8 * stage);
+            umma_commit_pair(bar_acc_full + 8 * buf);
+          } else {
+            umma_commit(bar_empty + 8 * stage);
+            umma_commit(bar_acc_full + 8 * buf);
+          }
+          if (++stage == F::kStages) { stage = 0; phase ^= 1u; }
+          if (++buf == F::kBufs) { buf = 0; buf_phase ^= 1u; }
+        }
+      }
+    }
+    __syncwarp();
+  }
+  } else {
+    if constexpr (kTn == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    // ---------------- epilogue warps: 32 lanes (rows) x kCols columns each, the outer sum in registers
+    constexpr int kCols = F::kCols;
+    const int sub = warp & 3, half = (warp - kFirstEpiWarp) >> 2;
+    float* strip = reinterpret_cast<float*>(base_ptr + kRingBytes + 256) + (warp - kFirstEpiWarp) * 2 * kCols;  // this warp's own
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    bool alive = true;
+    for (int item = first_item; item < items && alive; item += item_step) {
+      int tm, tn;
+      tile_of(item, tiles_m, tiles_n, max(kGroupM / kCg, 1), &tm, &tn);
+      const int row = (tm * kCg + (kCg == 2 ? static_cast<int>(rank) : 0)) * kTileM + sub * 32 + lane;
+      const int col0 = tn * kTn + half * kCols;
+      // scales: the row's, and either the one of this warp's 128-column block or one per column through the strip
+      const float* sa_ptr = p.sa.data + (row / p.sa.per) * p.sa.smn;
+      const float* sb_ptr = p.sb.data + (kVecB ? 0 : (col0 / kScaleBlk) * p.sb.smn);
+      const bool row_in = row < p.M, cols_in = col0 < p.N;
+      uint64_t acc[kCols / 2];
+#pragma unroll
+      for (int j = 0; j < kCols / 2; ++j) acc[j] = 0ull;
+      float sa_next = 0.0f, sb_next = 0.0f, vec_next[kCols / 32];
+      auto fetch = [&](int kb) {
+        sa_next = row_in ? __ldg(sa_ptr + kb * p.sa.sk) : 0.0f;
+        if constexpr (kVecB) {
+#pragma unroll
+          for (int h = 0; h < kCols / 32; ++h) {
+            const int col = col0 + lane + 32 * h;
+            vec_next[h] = col < p.N ? __ldg(sb_ptr + col * p.sb.smn + kb * p.sb.sk) : 0.0f;
+          }
+        } else {
+          sb_next = cols_in ? __ldg(sb_ptr + kb * p.sb.sk) : 0.0f;
+        }
+      };
+      fetch(kb_lo);
+      for (int kb = kb_lo; kb < kb_hi; ++kb) {
+        const float sa = sa_next, sb = sb_next;
+        const float* vec = strip + (kb & 1) * kCols;
+        if constexpr (kVecB) {
+#pragma unroll
+          for (int h = 0; h < kCols / 32; ++h) strip[(kb & 1) * kCols + lane + 32 * h] = vec_next[h];
+          __syncwarp();
+        }
+        if (kb + 1 < kb_hi) fetch(kb + 1);
+        // the MMA results and the TMEM loads are warp-collective: the whole warp proceeds or the whole warp leaves
+        if (!__all_sync(0xffffffffu, wait(bar_acc_full + 8 * buf, buf_phase, abort_flag, 4))) { alive = false; break; }
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + buf * kTn + half * kCols;
+        const float s = sa * sb;
+        const uint64_t s2 = pack2(s, s), sa2 = pack2(sa, sa), sb2 = pack2(sb, sb);
+        // the product of the two scales may leave fp32 where the scaled sum does not (a block of zeros, for one)
+        const bool one_factor = !kVecB && fabsf(s) <= 3.0e38f;
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld_32x32(taddr + 32 * c, r);
+          if (c == kCols / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (kCg == 2) mbar_arrive_cluster(map_to_cta(bar_acc_empty + 8 * buf, 0));
+              else mbar_arrive(bar_acc_empty + 8 * buf);
+            }
+          }
+          if constexpr (kVecB) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              const float4 b = *reinterpret_cast<const float4*>(vec + 32 * c + 2 * j);
+              const uint64_t d0 = pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+              const uint64_t d1 = pack2(__uint_as_float(r[2 * j + 2]), __uint_as_float(r[2 * j + 3]));
+              acc[16 * c + j] = fma2(mul2(d0, pack2(b.x, b.y)), sa2, acc[16 * c + j]);
+              acc[16 * c + j + 1] = fma2(mul2(d1, pack2(b.z, b.w)), sa2, acc[16 * c + j + 1]);
+            }
+          } else if (one_factor) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              acc[16 * c + j] = fma2(pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[16 * c + j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              acc[16 * c + j] = fma2(mul2(pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), sb2), sa2, acc[16 * c + j]);
+          }
+        }
+        if (++buf == F::kBufs) { buf = 0; buf_phase ^= 1u; }
+      }
+      if (!alive) break;
+      if (splits > 1) {
+        // this CTA's part of the sum, parked where the ring was: its last MMA has read it, and no load is in flight
+        float* park = reinterpret_cast<float*>(base_ptr) + (sub * 32 + lane) * (kTn + 4) + half * kCols;
+#pragma unroll
+        for (int j = 0; j < kCols / 2; j += 2) {
+          const float2 a = unpack2(acc[j]), b = unpack2(acc[j + 1]);
+          *reinterpret_cast<float4*>(park + 2 * j) = make_float4(a.x, a.y, b.x, b.y);
+        }
+        break;  // a split cluster has one item
+      }
+      if (p.bias_dtype != 0) {
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < kCols / 32; ++h) {
+          const int col = col0 + lane + 32 * h;
+          strip[lane + 32 * h] = col < p.N ? load_as_f32(p.bias, col * p.bias_stride, p.bias_dtype) : 0.0f;
+        }
+        __syncwarp();
+      }
+#pragma unroll
+      for (int c = 0; c < kCols / 32; ++c) {
+        if (col0 + 32 * c < p.N) {
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 a = unpack2(acc[16 * c + j]);
+            v[2 * j] = a.x, v[2 * j + 1] = a.y;
+          }
+          finish32(p, row, col0 + 32 * c, v, strip + 32 * c);
+        }
+      }
+      __syncwarp();
+    }
+  }
+
+  if constexpr (kCg == 1) {
+    if (splits > 1) {
+      // Every CTA of the cluster adds the parts of its share of the tile, in split order, and stores it.
+      cluster_sync_all();
+      if (warp >= kFirstEpiWarp) {
+        int tm, tn;
+        tile_of(first_item, tiles_m, tiles_n, kGroupM, &tm, &tn);
+        const int m0 = tm * kTileM, n0 = tn * kTn;
+        const int rows = min(kTileM, p.M - m0);
+        for (int i = static_cast<int>(rank) * (32 * kEpiWarps) + threadIdx.x - 32 * kFirstEpiWarp; i < rows * (kTn / 4); i += splits * 32 * kEpiWarps) {
+          const int r = i / (kTn / 4), c = (i % (kTn / 4)) * 4;
+          const uint32_t mine = base + (r * (kTn + 4) + c) * 4;
+          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int sp = 0; sp < splits; ++sp) {
+            float4 t;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(t.x), "=f"(t.y), "=f"(t.z), "=f"(t.w) : "r"(map_to_cta(mine, sp)) : "memory");
+            v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t row = m0 + r, col = n0 + c + e;
+            if (col >= p.N) break;
+            if (p.bias_dtype != 0) v[e] += load_as_f32(p.bias, col * p.bias_stride, p.bias_dtype);
+            if (p.relu && v[e] < 0.0f) v[e] = 0.0f;
+            if (p.mask && !(load_as_f32(p.mask, row * p.mask_ld + col, p.c_dtype) > 0.0f)) v[e] = 0.0f;
+            store_from_f32(p.C, row * p.ldc + col, p.c_dtype, v[e]);
+          }
+        }
+      }
+      cluster_sync_all();  // nobody leaves while a peer may still be reading its shared memory
+    }
+  }
+  if (*abort_flag) {
+    // error path only: give loads that may still be in flight time to land before shared memory is released
+    for (int i = 0; i < 64; ++i) __nanosleep(16384);
+  }
+  tc_fence_before();
+  if constexpr (kCg == 2) cluster_sync_all();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (kCg == 1) tmem_dealloc(tmem_base, F::kTmem);
+    else tmem_dealloc_pair(tmem_base, F::kTmem);
+  }
+}
+
+// Copies an operand to rows that start on 16 bytes. `wide`: source rows allow 4-byte loads.
+__global__ void __launch_bounds__(256) repitch_kernel(const uint8_t* __restrict__ src, int64_t rs, int64_t cs, int64_t rows, int64_t cols,
+                                                      uint8_t* __restrict__ dst, int64_t ld, int wide) {
+  const int64_t words = ld / 4;
+  const int64_t total = rows * words, stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
+    const int64_t r = i / words, c = (i % words) * 4;
+    const uint8_t* s = src + r * rs + c * cs;
+    uint32_t w = 0;
+    if (wide && c + 4 <= cols) {
+      w = *reinterpret_cast<const uint32_t*>(s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < cols) w |= static_cast<uint32_t>(s[e * cs]) << (8 * e);
+    }
+    *reinterpret_cast<uint32_t*>(dst + r * ld + c) = w;
+  }
+}
+
+// ------------------------------------------------------------------ host side
+// 0 = K-major, 1 = MN-major, -1 = TMA cannot address it as it is
+int operand_major(const MatView& v, bool k_is_row) {
+  const int64_t mn = k_is_row ? v.cols : v.rows, k = k_is_row ? v.rows : v.cols;
+  const int64_t mn_stride = k_is_row ? v.cs : v.rs, k_stride = k_is_row ? v.rs : v.cs;
+  if (!aligned_to(v.data, 16)) return -1;
+  if ((k == 1 || k_stride == 1) && (mn == 1 || (mn_stride % 16 == 0 && mn_stride >= k))) return 0;
+  if ((mn == 1 || mn_stride == 1) && (k == 1 || (k_stride % 16 == 0 && k_stride >= mn))) return 1;
+  return -1;
+}
+// An operand as the kernel reads it: `inner` contiguous elements per line, `outer` lines `ld` bytes apart.
+struct Operand {
+  const uint8_t* data;
+  int major;  // 0: inner = K, 1: inner = M / N
+  int64_t inner, outer, ld;
+  bool copied;
+  size_t copy_bytes;
+};
+Operand operand_of(const MatView& v, bool k_is_row) {
+  const int64_t mn = k_is_row ? v.cols : v.rows, k = k_is_row ? v.rows : v.cols;
+  const int64_t mn_stride = k_is_row ? v.cs : v.rs, k_stride = k_is_row ? v.rs : v.cs;
+  Operand o{static_cast<const uint8_t*>(v.data), operand_major(v, k_is_row), 0, 0, 0, false, 0};
+  o.copied = o.major < 0;
+  if (o.copied) o.major = mn_stride == 1 && k_stride != 1 ? 1 : 0;  // keeps the contiguous side contiguous
+  o.inner = o.major == 0 ? k : mn;
+  o.outer = o.major == 0 ? mn : k;
+  o.ld = o.major == 0 ? mn_stride : k_stride;
+  if (o.copied || o.outer == 1) o.ld = (o.inner + 15) / 16 * 16;
+  if (o.copied) o.copy_bytes = (static_cast<size_t>(o.outer) * o.ld + 255) / 256 * 256;
+  return o;
+}
+void repitch(const Operand& o, const MatView& v, bool k_is_row, uint8_t* dst, cudaStream_t stream) {
+  const int64_t mn_stride = k_is_row ? v.cs : v.rs, k_stride = k_is_row ? v.rs : v.cs;
+  const int64_t rs = o.major == 0 ? mn_stride : k_stride, cs = o.major == 0 ? k_stride : mn_stride;
+  const int wide = cs == 1 && rs % 4 == 0 && aligned_to(v.data, 4);
+  repitch_kernel<<<streaming_grid(o.outer * (o.ld / 4), 256, kStreamBlocksPerSm), 256, 0, stream>>>(
+      static_cast<const uint8_t*>(v.data), rs, cs, o.outer, o.inner, dst, o.ld, wide);
+}
+bool encode(CUtensorMap* map, const uint8_t* data, const Operand& o, uint32_t mn_box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(o.inner), static_cast<cuuint64_t>(o.outer)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(o.ld)};
+  const cuuint32_t box[2] = {128, o.major == 0 ? mn_box : static_cast<cuuint32_t>(kTileK)};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(data), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Choice {
+  int cg = 1, tn = 128, splits = 1;
+};
+// AICF_FP8_TILE=<ctas><columns>, e.g. 2256, 1256, 1128, 164; AICF_FP8_SPLITK=n: tuning, read on every launch
+Choice choose(const Fp8Problem& q) {
   const GemmProblem& g = q.g;
-  Fp8Params p{};
-  p.A = static_cast<const uint8_t*>(g.A.data);
-  p.B = static_cast<const uint8_t*>(g.B.data);
-  p.ars = g.A.rs, p.acs = g.A.cs, p.brs = g.B.rs, p.bcs = g.B.cs;
-  p.a_e5m2 = g.A.dtype == DType::kF8E5M2, p.b_e5m2 = g.B.dtype == DType::kF8E5M2;
-  p.sa = q.sa, p.sb = q.sb;
-  p.C = const_cast<void*>(g.C.data), p.ldc = g.C.rs, p.c_dtype = static_cast<int>(g.C.dtype);
-  p.bias = g.bias, p.bias_stride = g.bias_stride, p.bias_dtype = static_cast<int>(g.bias_dtype), p.relu = g.relu;
-  p.mask = g.mask, p.mask_ld = g.mask_ld;
-  p.M = static_cast<int>(g.M), p.N = static_cast<int>(g.N), p.K = static_cast<int>(g.K);
-  const int64_t tiles_m = (g.M + 63) / 64, tiles_n = (g.N + 63) / 64;
-  if (tiles_m > 0x7fffffff / tiles_n) return Status::InvalidArgument;
-  cudaGetLastError();
-  gemm_fp8_tile_kernel<<<static_cast<unsigned>(tiles_m * tiles_n), 256, 0, stream>>>(p, static_cast<int>(tiles_n));
+  Choice c;
+  const int64_t sms = sm_count(), kb = blocks_of(g.K);
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
+  if (g.M > 128 && tiles(256, 256) * 4 >= sms) c = Choice{2, 256, 1};
+  else c = Choice{1, 128, 1};
+  if (const char* e = std::getenv("AICF_FP8_TILE")) {
+    const int v = std::atoi(e);
+    if (v == 2256) c = Choice{2, 256, 1};
+    if (v == 1256) c = Choice{1, 256, 1};
+    if (v == 1128) c = Choice{1, 128, 1};
+    if (v == 164) c = Choice{1, 64, 1};
+  }
+  if (const char* e = std::getenv("AICF_FP8_SPLITK")) c.splits = std::atoi(e);
+  if (c.cg == 2 || c.tn == 256 || c.splits < 1) c.splits = 1;
+  while (c.splits > 1 && (c.splits > kb || (kb + c.splits - 1) / c.splits * (c.splits - 1) >= kb)) --c.splits;  // no empty part
+  return c;
+}
+
+template <int kCg, int kTn, bool kVecB>
+Status launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, const Fp8Params& p, cudaStream_t stream) {
+  using F = Cfg<kCg, kTn>;
+  auto kernel = gemm_fp8_kernel<kCg, kTn, kVecB>;
+  static PerDeviceOnce opt_in;
+  if (!opt_in.run([&] {
+        // a register hand-over that does not come out even would wait forever: refuse a build that has another count
+        cudaFuncAttributes a{};
+        return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && (kTn != 256 || a.numRegs == kRegsLaunch) &&
+               cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(F::kSmem)) == cudaSuccess;
+      })) {
+    cudaGetLastError();
+    return Status::Internal;
+  }
+  const int64_t items = ((static_cast<int64_t>(p.M) + kCg * kTileM - 1) / (kCg * kTileM)) * ((static_cast<int64_t>(p.N) + kTn - 1) / kTn);
+  if (items > 0x7fffffff / 8) return Status::InvalidArgument;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(kCg == 2 ? 2 : p.splits);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = F::kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = kCg == 2 || p.splits > 1 ? 1 : 0;
+  if (kCg == 2) {
+    const int64_t pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * (items < pairs ? items : pairs)));
+  } else if (p.splits > 1) {
+    cfg.gridDim = dim3(static_cast<unsigned>(items * p.splits));
+  } else {
+    cfg.gridDim = dim3(static_cast<unsigned>(items < sm_count() ? items : sm_count()));
+  }
+  if (cudaLaunchKernelEx(&cfg, kernel, ta, tb, p) != cudaSuccess) {
+    cudaGetLastError();
+    return Status::Internal;
+  }
   return launch_status();
 }
 
-size_t no_workspace(const TensorDesc*, int, const void*) { return 0; }
+Status run(const Fp8Problem& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  const GemmProblem& g = q.g;
+  if (!encode_fn()) return Status::NotImplemented;
+  // A is [M,K], B is [K,N]
+  const Operand a = operand_of(g.A, false), b = operand_of(g.B, true);
+  uint8_t* w = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
+  if (a.copied || b.copied) {
+    if (!ws || ws_bytes < a.copy_bytes + b.copy_bytes + 256) return Status::InvalidArgument;
+  }
+  cudaGetLastError();
+  if (a.copied) repitch(a, g.A, false, w, stream);
+  if (b.copied) repitch(b, g.B, true, w + a.copy_bytes, stream);
+
+  Choice c = choose(q);
+  if (c.tn == 64 && b.major == 1) c.tn = 128;  // an N-major box is 128 columns wide
+  CUtensorMap ta, tb;
+  if (!encode(&ta, a.copied ? w : a.data, a, kTileM) ||
+      !encode(&tb, b.copied ? w + a.copy_bytes : b.data, b, static_cast<uint32_t>(c.tn / c.cg)))
+    return Status::Internal;
+
+  Fp8Params p{};
+  p.C = const_cast<void*>(g.C.data);
+  p.ldc = g.M == 1 ? g.N : g.C.rs;
+  p.c_dtype = static_cast<int>(g.C.dtype);
+  const int64_t c_bytes = dtype_size_bytes(g.C.dtype);
+  p.c_vec = aligned_to(p.C, 32) && (p.ldc * c_bytes) % 32 == 0;
+  p.bias = g.bias;
+  p.bias_stride = g.bias_stride;
+  p.bias_dtype = g.bias ? static_cast<int>(g.bias_dtype) : 0;
+  p.relu = g.relu ? 1 : 0;
+  p.mask = g.mask;
+  p.mask_ld = g.mask_ld;
+  p.mask_vec = g.mask && aligned_to(g.mask, 16) && (g.mask_ld * c_bytes) % 16 == 0;
+  p.sa = q.sa;
+  p.sb = q.sb;
+  p.M = static_cast<int>(g.M), p.N = static_cast<int>(g.N), p.K = static_cast<int>(g.K);
+  p.a_mn_major = a.major, p.b_mn_major = b.major;
+  p.splits = c.splits;
+  // instruction descriptor: D = f32 (bits 4-5 = 1), A / B format (bits 7-9 / 10-12: 0 = e4m3, 1 = e5m2), A / B major
+  // (bits 15 / 16), N >> 3 (bits 17-22), M >> 4 (bits 24-28)
+  p.idesc = (1u << 4) | (g.A.dtype == DType::kF8E5M2 ? 1u << 7 : 0u) | (g.B.dtype == DType::kF8E5M2 ? 1u << 10 : 0u) |
+            (static_cast<uint32_t>(a.major) << 15) | (static_cast<uint32_t>(b.major) << 16) |
+            (static_cast<uint32_t>(c.tn >> 3) << 17) | (static_cast<uint32_t>((c.cg * kTileM) >> 4) << 24);
+  const bool vec = q.sb.per == 1;
+  if (c.cg == 2) return vec ? launch_tiles<2, 256, true>(ta, tb, p, stream) : launch_tiles<2, 256, false>(ta, tb, p, stream);
+  if (c.tn == 256) return vec ? launch_tiles<1, 256, true>(ta, tb, p, stream) : launch_tiles<1, 256, false>(ta, tb, p, stream);
+  if (c.tn == 128) return vec ? launch_tiles<1, 128, true>(ta, tb, p, stream) : launch_tiles<1, 128, false>(ta, tb, p, stream);
+  return vec ? launch_tiles<1, 64, true>(ta, tb, p, stream) : launch_tiles<1, 64, false>(ta, tb, p, stream);
+}
+
+// Bytes for the aligned copies of operands that TMA cannot address.
+template <Epi kEpi>
+size_t fp8_workspace(const TensorDesc* in, int ni, const void* attr) {
+  if (!in || ni < 4 || in[0].rank() != 2 || in[1].rank() != 2) return 0;
+  bool ta = false, tb = false, relu;
+  if (kEpi == Epi::BiasRelu) read_gemm_epilogue_attr(attr, &ta, &tb, &relu);
+  else read_gemm_attr(attr, &ta, &tb);
+  const Operand a = operand_of(view_of(in[0], ta), false), b = operand_of(view_of(in[1], tb), true);
+  return a.copied || b.copied ? a.copy_bytes + b.copy_bytes + 256 : 0;
+}
 
 template <DType kC, Epi kEpi>
 bool supported(const TensorDesc* in, int ni, const TensorDesc* out, int no, const void* attr) {
@@ -182,11 +780,25 @@ KernelVariant variant(const char* name) {
   v.flags = kKV_CaptureSafe;
   v.launch = launch<kC, kEpi>;
   v.supported = supported<kC, kEpi>;
-  v.query_workspace = no_workspace;
+  v.query_workspace = fp8_workspace<kEpi>;
   return v;
 }
 
 }  // namespace
+
+// Status word of the bounded waits, as gemm_tcgen05_status().
+int gemm_fp8_status(bool clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_fp8_status, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (clear && v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_fp8_status, &zero, sizeof(int));
+  }
+  return v;
+}
 
 KernelVariant make_gemm_fp8_block128_out_f32_variant() { return variant<DType::kF32, Epi::None>("gemm_fp8_block128_out_f32"); }
 KernelVariant make_gemm_fp8_block128_out_bf16_variant() { return variant<DType::kBF16, Epi::None>("gemm_fp8_block128_out_bf16"); }
