@@ -89,13 +89,8 @@ constexpr int kTileK = 128;        // bytes of K per stage: one scale block, one
 constexpr int kUmmaK = 32;         // k extent of one kind::f8f6f4 MMA
 constexpr int kChunkBytes = kTileK * 128;   // MN-major operands: 128 k rows of 128 bytes
 constexpr int kRingBytes = 192 * 1024;
-constexpr int kEpiWarps = 8;
-constexpr int kFirstEpiWarp = 4;   // warps 2 and 3 have no work: they complete the first warpgroup
-constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
-// The 256-column tile holds 128 fp32 sums per epilogue thread. 384 threads are launched with 168 registers each; the first
-// warpgroup gives up 128 of its own and the two epilogue warpgroups take 64 more: 128 * 40 + 256 * 232 = 384 * 168.
-constexpr int kRegsLaunch = 168, kRegsRoles = 40, kRegsEpi = 232;
-static_assert(128 * kRegsRoles + 32 * kEpiWarps * kRegsEpi <= kThreads * kRegsLaunch, "the warpgroups' shares come out of the block's registers");
+constexpr int kFirstEpiWarp = 4;   // warps 0-3: TMA, MMA, scales, scales
+constexpr int kScaleGroup = 8;     // k blocks whose scales are staged at a time
 constexpr int kGroupM = 16;        // tile rasterisation: 16 row tiles share their column tiles in L2
 constexpr unsigned long long kWaitBudgetNs = 1000000000ull;
 
@@ -111,6 +106,7 @@ struct Fp8Params {
   int c_dtype, bias_dtype;  // DType values, 0 = no bias
   int relu;
   int c_vec, mask_vec;   // rows of C (of the mask) allow 32-byte stores (16-byte loads)
+  int bias_vec;          // fp32, unit stride, 16-byte aligned
   int a_mn_major, b_mn_major;
   uint32_t idesc;
   int splits;            // CTAs of a cluster that share a tile, each with a range of k blocks (single-CTA kernel)
@@ -118,21 +114,47 @@ struct Fp8Params {
 
 // Tile shapes. kCg CTAs work on one tile of kCg * 128 rows and kTn columns; each holds 128 rows of A and kTn / kCg columns of
 // B per stage, and a 128 x kTn accumulator.
-template <int kCg, int kTn> struct Cfg {
+template <int kCg, int kTn, bool kVecB> struct Cfg {
   static constexpr int kBCols = kTn / kCg;
   static constexpr int kABytes = kTileM * kTileK;
   static constexpr int kStageBytes = kABytes + kBCols * kTileK;
   static constexpr int kStages = kRingBytes / kStageBytes;
   static constexpr int kBufs = kTn == 256 ? 2 : 4;          // accumulator buffers in tensor memory
   static constexpr int kTmem = kBufs * kTn;
-  static constexpr int kCols = kTn / 2;                     // columns per epilogue warp
-  static constexpr size_t kStripBytes = size_t(kEpiWarps) * 2 * kCols * sizeof(float);
-  static constexpr size_t kSmem = 1024 + kRingBytes + 256 + kStripBytes;
-  static_assert(16 * kStages + 16 * kBufs + 8 <= 256, "barriers fit their 256 bytes");
+  // Epilogue warps: two per 32 rows, half the tile's columns each. For the 256-column tile that is 128 fp32 sums a thread:
+  // 384 threads are launched with 168 registers each, the first warpgroup gives up 128 of its own and the epilogue
+  // warpgroups take 64 more: 128 * 40 + 256 * 232 = 384 * 168. (Sixteen warps of 64 columns spill at the 112 registers they
+  // could have, and were slower: 1657 against 524 us at 8192^3.)
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
+  static constexpr bool kRegShift = kTn == 256;
+  static constexpr int kRegsLaunch = 168, kRegsRoles = 40, kRegsEpi = 232;
+  static_assert(128 * kRegsRoles + 32 * kEpiWarps * kRegsEpi <= kThreads * kRegsLaunch, "the warpgroups' shares come out of the block's registers");
+  static constexpr int kCols = kTn / (kEpiWarps / 4);       // columns per epilogue warp
+    static constexpr int kCh = 16;                                   // columns per TMEM load
+  // staged scales: two groups of kScaleGroup k blocks, each the rows' and then the columns' factors
+  static constexpr int kColScales = kVecB ? kTn : 2;        // one per column, or one per 128-column block of the tile
+  static constexpr int kGroupFloats = kScaleGroup * (kTileM + kColScales) + 4;  // the last four: one flag per scale warp, padding
+  static constexpr size_t kSmem = 1024 + kRingBytes + 256 + 2 * kGroupFloats * sizeof(float);
+  static_assert(kBufs <= kStages, "one parity per block in flight");
+  static_assert(16 * kStages + 8 * kBufs + 32 + 8 <= 256, "barriers fit their 256 bytes");
 };
 
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
-  return mbar_wait_or_abort(bar, parity, abort_flag, &g_fp8_status, who, kWaitBudgetNs);
+// Bounded wait of a whole warp: every lane leaves with the same answer. The clock behind the bound is read only after some
+// tries: reading it costs more than a wait usually lasts.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
+  for (int i = 0; i < 32; ++i)
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, abort_flag, &g_fp8_status, who, kWaitBudgetNs));
+}
+// True in one lane of a converged warp. The producer's and the issuer's loops run in the whole warp, so that addresses and
+// descriptors stay in uniform registers, and only the asynchronous instructions are left to this lane: with the loop itself
+// behind `lane == 0` every operand is moved to a uniform register first, and issuing one block's four MMAs and two commits
+// took 630 cycles, more than executing them.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
 }
 template <int kCg>
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -149,6 +171,37 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, int mn_major) {
   const uint64_t lbo = mn_major ? (kChunkBytes >> 4) : 1;
   return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (lbo << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// kN (32 or 16) consecutive columns of this warp's 32 lanes; the registers may be read after tmem_ld_wait only.
+template <int kN>
+__device__ __forceinline__ void tmem_ld_start(uint32_t taddr, uint32_t (&r)[kN]) {
+  if constexpr (kN == 32)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Waits for this warp's loads; naming the registers keeps their uses behind the wait.
+template <int kN>
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[kN]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < kN; ++j) asm volatile("" : "+r"(r[j]));
 }
 
 // Packed fp32 pairs: Blackwell's FMA pipe takes two per instruction.
@@ -189,11 +242,19 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t* w) {
                ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
-// 32 consecutive columns of one row of C: bias (from shared memory) and ReLU, or the ReLU-backward mask; convert; store.
-__device__ __forceinline__ void finish32(const Fp8Params& p, int row, int col0, float (&v)[32], const float* bias) {
-  if (p.bias_dtype != 0) {
+// 32 consecutive columns of one row of C: bias and ReLU, or the ReLU-backward mask; convert; store.
+__device__ __forceinline__ void finish32(const Fp8Params& p, int row, int col0, float (&v)[32]) {
+  if (p.bias_vec && col0 + 32 <= p.N) {  // the same address in every lane
+    const float4* b = reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + col0);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += bias[j];
+    for (int q = 0; q < 8; ++q) {
+      const float4 t = __ldg(b + q);
+      v[4 * q] += t.x, v[4 * q + 1] += t.y, v[4 * q + 2] += t.z, v[4 * q + 3] += t.w;
+    }
+  } else if (p.bias_dtype != 0) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < p.N) v[j] += load_as_f32(p.bias, (col0 + j) * p.bias_stride, p.bias_dtype);
   }
   if (p.relu) {
 #pragma unroll
@@ -281,16 +342,19 @@ __device__ __forceinline__ void tile_of(int item, int tiles_m, int tiles_n, int 
 
 // kVecB: the columns of B have a scale each (per = 1); otherwise 128 columns share one.
 template <int kCg, int kTn, bool kVecB>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<kCg, kTn, kVecB>::kThreads, 1)
     gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const Fp8Params p) {
-  using F = Cfg<kCg, kTn>;
+  using F = Cfg<kCg, kTn, kVecB>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;  // 128B swizzle atoms repeat every 1024 B
   uint8_t* base_ptr = smem_raw + (base - raw);
-  const uint32_t bar_full = base + kRingBytes, bar_empty = bar_full + 8 * F::kStages, bar_acc_full = bar_empty + 8 * F::kStages,
-                 bar_acc_empty = bar_acc_full + 8 * F::kBufs;
-  uint8_t* misc = base_ptr + kRingBytes + 16 * F::kStages + 16 * F::kBufs;
+  // bar_empty[stage] is the completion of a k block's MMAs: the producer takes it as "stage free" and the epilogue as
+  // "accumulator ready". The issuer is at most kBufs < kStages blocks ahead of the epilogue, so a parity names one block.
+  const uint32_t bar_full = base + kRingBytes, bar_empty = bar_full + 8 * F::kStages,
+                 bar_acc_empty = bar_empty + 8 * F::kStages, bar_sc_full = bar_acc_empty + 8 * F::kBufs, bar_sc_empty = bar_sc_full + 16;
+  uint8_t* misc = base_ptr + kRingBytes + 16 * F::kStages + 8 * F::kBufs + 32;
+  float* scales = reinterpret_cast<float*>(base_ptr + kRingBytes + 256);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
 
@@ -313,9 +377,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
     }
-    for (int b = 0; b < F::kBufs; ++b) {
-      mbar_init(bar_acc_full + 8 * b, 1);
-      mbar_init(bar_acc_empty + 8 * b, kCg * kEpiWarps);
+    for (int b = 0; b < F::kBufs; ++b) mbar_init(bar_acc_empty + 8 * b, kCg * F::kEpiWarps);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(bar_sc_full + 8 * g, 2);           // the two scale warps
+      mbar_init(bar_sc_empty + 8 * g, F::kEpiWarps);
     }
     *abort_flag = 0;
     mbar_init_fence();
@@ -332,10 +397,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp < kFirstEpiWarp) {
-  if constexpr (kTn == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRoles));
+  if constexpr (F::kRegShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::kRegsRoles));
   if (warp == 0) {
     // ---------------- TMA producer: in a pair each CTA loads its own halves, completion lands on the leader's barrier
-    if (lane == 0) {
+    {
       int stage = 0;
       uint32_t phase = 0;
       bool alive = true;
@@ -345,11 +410,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int m0 = (tm * kCg + (kCg == 2 ? static_cast<int>(rank) : 0)) * kTileM;
         const int n0 = tn * kTn + (kCg == 2 ? static_cast<int>(rank) * F::kBCols : 0);
         for (int kb = kb_lo; kb < kb_hi; ++kb) {
-          if (!wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, 1)) { alive = false; break; }
+          if (!warp_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, 1)) { alive = false; break; }
           const uint32_t sa = base + stage * F::kStageBytes, sb = sa + F::kABytes;
           const int k0 = kb * kTileK;
           const int ax = p.a_mn_major ? m0 : k0, ay = p.a_mn_major ? k0 : m0;
           const int bx = p.b_mn_major ? n0 : k0, by = p.b_mn_major ? k0 : n0;
+          if (elect_one()) {
           if constexpr (kCg == 2) {
             const uint32_t full = map_to_cta(bar_full + 8 * stage, 0);
             if (leader) mbar_expect_tx(bar_full + 8 * stage, 2 * F::kStageBytes);
@@ -362,6 +428,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_2d(sb, &tmap_b, bx, by, full);
             if (kTn == 256 && p.b_mn_major) tma_load_2d(sb + kChunkBytes, &tmap_b, bx + 128, by, full);
           }
+          }
+          __syncwarp();
           if (++stage == F::kStages) { stage = 0; phase ^= 1u; }
         }
       }
@@ -369,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA issuer: one lane, in a pair the leader's
-    if (leader && lane == 0) {
+    if (leader) {
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       bool alive = true;
@@ -377,112 +445,195 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t b_step = p.b_mn_major ? (kUmmaK * 128) >> 4 : kUmmaK >> 4;
       for (int item = first_item; item < items && alive; item += item_step) {
         for (int kb = kb_lo; kb < kb_hi; ++kb) {
-          if (!wait(bar_acc_empty + 8 * buf, buf_phase ^ 1u, abort_flag, 2)) { alive = false; break; }
-          if (!wait(bar_full + 8 * stage, phase, abort_flag, 3)) { alive = false; break; }
+          const uint32_t both = mbar_try_wait(bar_acc_empty + 8 * buf, buf_phase ^ 1u) & mbar_try_wait(bar_full + 8 * stage, phase);
+          if (!__all_sync(0xffffffffu, both)) {
+            if (!warp_wait(bar_acc_empty + 8 * buf, buf_phase ^ 1u, abort_flag, 2) || !warp_wait(bar_full + 8 * stage, phase, abort_flag, 3)) {
+              alive = false;
+              break;
+            }
+          }
           tc_fence_after();
           const uint32_t sa = base + stage * F::kStageBytes, sb = sa + F::kABytes;
           const uint64_t adesc = smem_desc(sa, p.a_mn_major), bdesc = smem_desc(sb, p.b_mn_major);
+          if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < kTileK / kUmmaK; ++k)
             umma_f8<kCg>(tmem_base + buf * kTn, adesc + k * a_step, bdesc + k * b_step, p.idesc, k != 0 ? 1u : 0u);
           if constexpr (kCg == 2) {
             umma_commit_pair(bar_empty + 8 * stage);
-            umma_commit_pair(bar_acc_full + 8 * buf);
           } else {
             umma_commit(bar_empty + 8 * stage);
-            umma_commit(bar_acc_full + 8 * buf);
           }
+          }
+          __syncwarp();
           if (++stage == F::kStages) { stage = 0; phase ^= 1u; }
           if (++buf == F::kBufs) { buf = 0; buf_phase ^= 1u; }
         }
       }
     }
     __syncwarp();
+  } else {
+    // ---------------- scales: both warps stage the factors of kScaleGroup k blocks at a time, two groups ahead at most.
+    // Read where they are used, a row's factor would cost its warp an uncoalesced load (32 rows, 32 sectors) per k block.
+    const int t = threadIdx.x - 64;
+    int g = 0;
+    uint32_t g_phase = 0;
+    bool alive = true;
+    for (int item = first_item; item < items && alive; item += item_step) {
+      int tm, tn;
+      tile_of(item, tiles_m, tiles_n, max(kGroupM / kCg, 1), &tm, &tn);
+      const int m0 = (tm * kCg + (kCg == 2 ? static_cast<int>(rank) : 0)) * kTileM, n0 = tn * kTn;
+      for (int kb0 = kb_lo; kb0 < kb_hi; kb0 += kScaleGroup) {
+        if (!warp_wait(bar_sc_empty + 8 * g, g_phase ^ 1u, abort_flag, 5)) { alive = false; break; }
+        float* rows_s = scales + g * F::kGroupFloats;
+        float* cols_s = rows_s + kScaleGroup * kTileM;
+        const int n = min(kScaleGroup, kb_hi - kb0);
+        float row_max = 0.0f, col_max = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = m0 + t + 64 * h;
+          const float* src = p.sa.data + (row / p.sa.per) * p.sa.smn + kb0 * p.sa.sk;
+#pragma unroll
+          for (int q = 0; q < kScaleGroup; ++q) {
+            const float f = row < p.M && q < n ? __ldg(src + q * p.sa.sk) : 0.0f;
+            rows_s[q * kTileM + t + 64 * h] = f;
+            row_max = fmaxf(row_max, fabsf(f));
+          }
+        }
+        if constexpr (kVecB) {
+#pragma unroll
+          for (int h = 0; h < kTn / 64; ++h) {
+            const int col = n0 + t + 64 * h;
+            const float* src = p.sb.data + col * p.sb.smn + kb0 * p.sb.sk;
+#pragma unroll
+            for (int q = 0; q < kScaleGroup; ++q)
+              cols_s[q * kTn + t + 64 * h] = col < p.N && q < n ? __ldg(src + q * p.sb.sk) : 0.0f;
+          }
+        } else {
+          const int q = (t & 15) >> 1, blk = n0 / kScaleBlk + (t & 1);  // a tile narrower than 128 columns lies in one block
+          const float f = blk * kScaleBlk < p.N && q < n ? __ldg(p.sb.data + blk * p.sb.smn + (kb0 + q) * p.sb.sk) : 0.0f;
+          if (t < 2 * kScaleGroup) cols_s[t] = f;
+          // The product of two scales may leave fp32 where the scaled sum does not (a block of zeros, for one): then the
+          // group is scaled by one factor after the other.
+          row_max = warp_max(row_max);
+          col_max = warp_max(fabsf(f));
+          if (lane == 0) rows_s[F::kGroupFloats - 4 + (t >> 5)] = row_max * col_max <= 3.0e38f ? 0.0f : 1.0f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_sc_full + 8 * g);
+        if (++g == 2) { g = 0; g_phase ^= 1u; }
+      }
+    }
   }
   } else {
-    if constexpr (kTn == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    if constexpr (F::kRegShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::kRegsEpi));
     // ---------------- epilogue warps: 32 lanes (rows) x kCols columns each, the outer sum in registers
     constexpr int kCols = F::kCols;
     const int sub = warp & 3, half = (warp - kFirstEpiWarp) >> 2;
-    float* strip = reinterpret_cast<float*>(base_ptr + kRingBytes + 256) + (warp - kFirstEpiWarp) * 2 * kCols;  // this warp's own
-    int buf = 0;
-    uint32_t buf_phase = 0;
+    int buf = 0, stage = 0, g = 0;
+    uint32_t phase = 0, g_phase = 0;
     bool alive = true;
+    const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + half * kCols;
     for (int item = first_item; item < items && alive; item += item_step) {
       int tm, tn;
       tile_of(item, tiles_m, tiles_n, max(kGroupM / kCg, 1), &tm, &tn);
       const int row = (tm * kCg + (kCg == 2 ? static_cast<int>(rank) : 0)) * kTileM + sub * 32 + lane;
       const int col0 = tn * kTn + half * kCols;
-      // scales: the row's, and either the one of this warp's 128-column block or one per column through the strip
-      const float* sa_ptr = p.sa.data + (row / p.sa.per) * p.sa.smn;
-      const float* sb_ptr = p.sb.data + (kVecB ? 0 : (col0 / kScaleBlk) * p.sb.smn);
-      const bool row_in = row < p.M, cols_in = col0 < p.N;
       uint64_t acc[kCols / 2];
 #pragma unroll
       for (int j = 0; j < kCols / 2; ++j) acc[j] = 0ull;
-      float sa_next = 0.0f, sb_next = 0.0f, vec_next[kCols / 32];
-      auto fetch = [&](int kb) {
-        sa_next = row_in ? __ldg(sa_ptr + kb * p.sa.sk) : 0.0f;
-        if constexpr (kVecB) {
+      // A buffer is read in chunks of kCh columns through two register sets: while a chunk is scaled and added the next one
+      // is on its way, and the first one of the next buffer while the last one of this is. The loop is rotated so that
+      // every load stands at one place in it: a register set that is loaded at two places costs a copy per register.
+      constexpr int kCh = F::kCh, kChunks = kCols / kCh;
+      static_assert(kChunks % 2 == 0, "chunk c uses register set c & 1");
+      uint32_t r[2][kCh];
+      // One chunk scaled and added: by the row's factor `f`, and the columns' factors `vec` (kVecB) or, in a group whose
+      // scales multiply out of range (kApart), the block's factor `g` first.
+      auto add_chunk = [&](auto apart, int c, float f, float fb, const float* vec) {
+        constexpr bool kApart = decltype(apart)::value;
+        const uint32_t(&d)[kCh] = r[c & 1];
+        const uint64_t f2 = pack2(f, f), fb2 = pack2(fb, fb);
 #pragma unroll
-          for (int h = 0; h < kCols / 32; ++h) {
-            const int col = col0 + lane + 32 * h;
-            vec_next[h] = col < p.N ? __ldg(sb_ptr + col * p.sb.smn + kb * p.sb.sk) : 0.0f;
+        for (int j = 0; j < kCh / 2; j += 2) {
+          uint64_t d0 = pack2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1]));
+          uint64_t d1 = pack2(__uint_as_float(d[2 * j + 2]), __uint_as_float(d[2 * j + 3]));
+          if constexpr (kVecB) {
+            const float4 b = *reinterpret_cast<const float4*>(vec + kCh * c + 2 * j);
+            d0 = mul2(d0, pack2(b.x, b.y));
+            d1 = mul2(d1, pack2(b.z, b.w));
+          } else if constexpr (kApart) {
+            d0 = mul2(d0, fb2);
+            d1 = mul2(d1, fb2);
           }
-        } else {
-          sb_next = cols_in ? __ldg(sb_ptr + kb * p.sb.sk) : 0.0f;
+          acc[kCh / 2 * c + j] = fma2(d0, f2, acc[kCh / 2 * c + j]);
+          acc[kCh / 2 * c + j + 1] = fma2(d1, f2, acc[kCh / 2 * c + j + 1]);
         }
       };
-      fetch(kb_lo);
-      for (int kb = kb_lo; kb < kb_hi; ++kb) {
-        const float sa = sa_next, sb = sb_next;
-        const float* vec = strip + (kb & 1) * kCols;
-        if constexpr (kVecB) {
+      // The k blocks of one scale group. Everything a block needs before its first load - its barrier, its factors - is asked
+      // for while the block before it is still being added: asked for at the loop's top, their latencies alone came to
+      // about as much as the block's MMAs take.
+      auto run_group = [&](auto apart, int n) {
+        const float* rows_s = scales + g * F::kGroupFloats + sub * 32 + lane;
+        const float* cols_s = scales + g * F::kGroupFloats + kScaleGroup * kTileM + (kVecB ? half * kCols : (half * kCols) / kScaleBlk);
+        constexpr bool kOne = !kVecB && !decltype(apart)::value;  // both scales in one factor
+        float f = 0.0f, fb = 0.0f;
+        const float* vec = cols_s;
 #pragma unroll
-          for (int h = 0; h < kCols / 32; ++h) strip[(kb & 1) * kCols + lane + 32 * h] = vec_next[h];
+        for (int j = 0; j < kCh; ++j) r[1][j] = 0u;  // "last chunk" before the group's first block: adds zeros
+        float row_f = rows_s[0], col_f = kVecB ? 1.0f : cols_s[0];
+        uint32_t ready = mbar_try_wait(bar_empty + 8 * stage, phase);
+#pragma unroll 1
+        for (int q = 0; q < n; ++q) {
+          // the TMEM loads are warp-collective: the whole warp proceeds or the whole warp leaves
+          if (!__all_sync(0xffffffffu, ready) && !warp_wait(bar_empty + 8 * stage, phase, abort_flag, 4)) return false;
+          tc_fence_after();
+          const uint32_t tbuf = tmem_lane + buf * kTn;
+          tmem_ld_start<kCh>(tbuf, r[0]);
+          add_chunk(apart, kChunks - 1, f, fb, vec);
+          f = kOne ? row_f * col_f : row_f;
+          fb = col_f;
+          vec = cols_s + q * kTn;
+          const uint32_t empty = bar_acc_empty + 8 * buf;
+          if (++buf == F::kBufs) buf = 0;
+          if (++stage == F::kStages) { stage = 0; phase ^= 1u; }
+#pragma unroll
+          for (int c = 0; c + 1 < kChunks; ++c) {
+            tmem_ld_wait<kCh>(r[c & 1]);
+            tmem_ld_start<kCh>(tbuf + kCh * (c + 1), r[(c + 1) & 1]);
+            if (c + 2 == kChunks) {
+              const int next = q + 1 < n ? q + 1 : q;
+              row_f = rows_s[next * kTileM];
+              if (!kVecB) col_f = cols_s[2 * next];
+              ready = mbar_try_wait(bar_empty + 8 * stage, phase);
+            }
+            add_chunk(apart, c, f, fb, vec);
+          }
+          tmem_ld_wait<kCh>(r[1]);
+          tc_fence_before();
           __syncwarp();
-        }
-        if (kb + 1 < kb_hi) fetch(kb + 1);
-        // the MMA results and the TMEM loads are warp-collective: the whole warp proceeds or the whole warp leaves
-        if (!__all_sync(0xffffffffu, wait(bar_acc_full + 8 * buf, buf_phase, abort_flag, 4))) { alive = false; break; }
-        tc_fence_after();
-        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + buf * kTn + half * kCols;
-        const float s = sa * sb;
-        const uint64_t s2 = pack2(s, s), sa2 = pack2(sa, sa), sb2 = pack2(sb, sb);
-        // the product of the two scales may leave fp32 where the scaled sum does not (a block of zeros, for one)
-        const bool one_factor = !kVecB && fabsf(s) <= 3.0e38f;
-#pragma unroll
-        for (int c = 0; c < kCols / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld_32x32(taddr + 32 * c, r);
-          if (c == kCols / 32 - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (kCg == 2) mbar_arrive_cluster(map_to_cta(bar_acc_empty + 8 * buf, 0));
-              else mbar_arrive(bar_acc_empty + 8 * buf);
-            }
-          }
-          if constexpr (kVecB) {
-#pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              const float4 b = *reinterpret_cast<const float4*>(vec + 32 * c + 2 * j);
-              const uint64_t d0 = pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-              const uint64_t d1 = pack2(__uint_as_float(r[2 * j + 2]), __uint_as_float(r[2 * j + 3]));
-              acc[16 * c + j] = fma2(mul2(d0, pack2(b.x, b.y)), sa2, acc[16 * c + j]);
-              acc[16 * c + j + 1] = fma2(mul2(d1, pack2(b.z, b.w)), sa2, acc[16 * c + j + 1]);
-            }
-          } else if (one_factor) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              acc[16 * c + j] = fma2(pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[16 * c + j]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              acc[16 * c + j] = fma2(mul2(pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), sb2), sa2, acc[16 * c + j]);
+          if (lane == 0) {
+            if constexpr (kCg == 2) mbar_arrive_cluster(map_to_cta(empty, 0));
+            else mbar_arrive(empty);
           }
         }
-        if (++buf == F::kBufs) { buf = 0; buf_phase ^= 1u; }
+        add_chunk(apart, kChunks - 1, f, fb, vec);
+        return true;
+      };
+#pragma unroll 1
+      for (int kb0 = kb_lo; kb0 < kb_hi && alive; kb0 += kScaleGroup) {
+        alive = warp_wait(bar_sc_full + 8 * g, g_phase, abort_flag, 6);
+        if (!alive) break;
+        const int n = min(kScaleGroup, kb_hi - kb0);
+        if constexpr (kVecB) {
+          alive = run_group(std::false_type{}, n);
+        } else {
+          const float2 flags = *reinterpret_cast<const float2*>(scales + (g + 1) * F::kGroupFloats - 4);
+          alive = flags.x + flags.y == 0.0f ? run_group(std::false_type{}, n) : run_group(std::true_type{}, n);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_sc_empty + 8 * g);
+        if (++g == 2) { g = 0; g_phase ^= 1u; }
       }
       if (!alive) break;
       if (splits > 1) {
@@ -495,15 +646,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         break;  // a split cluster has one item
       }
-      if (p.bias_dtype != 0) {
-        __syncwarp();
-#pragma unroll
-        for (int h = 0; h < kCols / 32; ++h) {
-          const int col = col0 + lane + 32 * h;
-          strip[lane + 32 * h] = col < p.N ? load_as_f32(p.bias, col * p.bias_stride, p.bias_dtype) : 0.0f;
-        }
-        __syncwarp();
-      }
 #pragma unroll
       for (int c = 0; c < kCols / 32; ++c) {
         if (col0 + 32 * c < p.N) {
@@ -513,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float2 a = unpack2(acc[16 * c + j]);
             v[2 * j] = a.x, v[2 * j + 1] = a.y;
           }
-          finish32(p, row, col0 + 32 * c, v, strip + 32 * c);
+          finish32(p, row, col0 + 32 * c, v);
         }
       }
       __syncwarp();
@@ -529,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tile_of(first_item, tiles_m, tiles_n, kGroupM, &tm, &tn);
         const int m0 = tm * kTileM, n0 = tn * kTn;
         const int rows = min(kTileM, p.M - m0);
-        for (int i = static_cast<int>(rank) * (32 * kEpiWarps) + threadIdx.x - 32 * kFirstEpiWarp; i < rows * (kTn / 4); i += splits * 32 * kEpiWarps) {
+        for (int i = static_cast<int>(rank) * (32 * F::kEpiWarps) + threadIdx.x - 32 * kFirstEpiWarp; i < rows * (kTn / 4); i += splits * 32 * F::kEpiWarps) {
           const int r = i / (kTn / 4), c = (i % (kTn / 4)) * 4;
           const uint32_t mine = base + (r * (kTn + 4) + c) * 4;
           float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -662,13 +804,13 @@ Choice choose(const Fp8Problem& q) {
 
 template <int kCg, int kTn, bool kVecB>
 Status launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, const Fp8Params& p, cudaStream_t stream) {
-  using F = Cfg<kCg, kTn>;
+  using F = Cfg<kCg, kTn, kVecB>;
   auto kernel = gemm_fp8_kernel<kCg, kTn, kVecB>;
   static PerDeviceOnce opt_in;
   if (!opt_in.run([&] {
         // a register hand-over that does not come out even would wait forever: refuse a build that has another count
         cudaFuncAttributes a{};
-        return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && (kTn != 256 || a.numRegs == kRegsLaunch) &&
+        return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && (!F::kRegShift || a.numRegs == F::kRegsLaunch) &&
                cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(F::kSmem)) == cudaSuccess;
       })) {
     cudaGetLastError();
@@ -682,7 +824,7 @@ Status launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, const Fp8Param
   attr[0].val.clusterDim.x = static_cast<unsigned>(kCg == 2 ? 2 : p.splits);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(F::kThreads);
   cfg.dynamicSmemBytes = F::kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -731,6 +873,7 @@ Status run(const Fp8Problem& q, void* ws, size_t ws_bytes, cudaStream_t stream) 
   p.bias = g.bias;
   p.bias_stride = g.bias_stride;
   p.bias_dtype = g.bias ? static_cast<int>(g.bias_dtype) : 0;
+  p.bias_vec = g.bias && g.bias_dtype == DType::kF32 && g.bias_stride == 1 && aligned_to(g.bias, 16);
   p.relu = g.relu ? 1 : 0;
   p.mask = g.mask;
   p.mask_ld = g.mask_ld;
