@@ -13,6 +13,7 @@ namespace aicf::cuda {
 int gemm_tcgen05_status(bool clear);
 int gemm_fp8_status(bool clear);
 int row_pipeline_status(bool clear);
+int distill_pipeline_status(bool clear);
 int layernorm_pipeline_status(bool clear);
 int adam_pipeline_status(bool clear);
 int gemm_tcgen05_timeline(int enable, unsigned long long* out16);
@@ -253,11 +254,12 @@ int aicf_b200_gemm_timeline(int enable, uint64_t* out16) {
 int aicf_b200_wait_status(int clear) {
   const int g = aicf_b200_gemm_status(clear);
   const int rs = aicf::cuda::row_pipeline_status(clear != 0);
+  const int rk = aicf::cuda::distill_pipeline_status(clear != 0);
   const int rl = aicf::cuda::layernorm_pipeline_status(clear != 0);
   const int ra = aicf::cuda::adam_pipeline_status(clear != 0);
   const int d = aicf::cuda::dp_wait_status(clear != 0);
-  if (g < 0 || rs < 0 || rl < 0 || ra < 0 || d < 0) return -1;
-  const int r = rs | rl | ra;
+  if (g < 0 || rs < 0 || rk < 0 || rl < 0 || ra < 0 || d < 0) return -1;
+  const int r = rs | rk | rl | ra;
   return (g & 0xFFFF) | (r ? 0x10000 : 0) | ((d & 3) << 17);
 }
 

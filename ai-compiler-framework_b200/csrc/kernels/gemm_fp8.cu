@@ -122,13 +122,13 @@ template <int kCg, int kTn, bool kVecB> struct Cfg {
   static constexpr int kBufs = kTn == 256 ? 2 : 4;          // accumulator buffers in tensor memory
   static constexpr int kTmem = kBufs * kTn;
   // Epilogue warps: two per 32 rows, half the tile's columns each. For the 256-column tile that is 128 fp32 sums a thread:
-  // 384 threads are launched with 168 registers each, the first warpgroup gives up 128 of its own and the epilogue
-  // warpgroups take 64 more: 128 * 40 + 256 * 232 = 384 * 168. (Sixteen warps of 64 columns spill at the 112 registers they
+  // 384 threads are launched with 168 registers each, the first warpgroup gives up 112 of its own and the epilogue
+  // warpgroups take 56 more: 128 * 56 + 256 * 224 = 384 * 168. (Sixteen warps of 64 columns spill at the 112 registers they
   // could have, and were slower: 1657 against 524 us at 8192^3.)
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
   static constexpr bool kRegShift = kTn == 256;
-  static constexpr int kRegsLaunch = 168, kRegsRoles = 40, kRegsEpi = 232;
+  static constexpr int kRegsLaunch = 168, kRegsRoles = 56, kRegsEpi = 224;
   static_assert(128 * kRegsRoles + 32 * kEpiWarps * kRegsEpi <= kThreads * kRegsLaunch, "the warpgroups' shares come out of the block's registers");
   static constexpr int kCols = kTn / (kEpiWarps / 4);       // columns per epilogue warp
     static constexpr int kCh = 16;                                   // columns per TMEM load
