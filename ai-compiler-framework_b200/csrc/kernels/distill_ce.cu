@@ -147,6 +147,16 @@ __global__ void __launch_bounds__(256) distill_multipass_kernel(const DistillPar
 }
 
 // ------------------------------------------------------------------ one read, one write
+// Exponentials are taken in powers of two: with c = log2(e) / T and n = max(z) c, rounded to fp32, softmax(z / T) is
+// 2^(z c - n) / S, S the sum of the numerators. z c - n is one fused multiply-add, so n is an exact reference and a logit
+// costs three instructions. The three kinds of row differ in who holds it:
+//
+//   distill_warp_kernel    up to 2048 columns: one warp per row, the row in its registers, many short blocks
+//   distill_block_kernel   longer rows: one CTA, or one per slice of the row in a cluster, the slice in shared memory
+//   distill_multipass_kernel  z and dz misaligned against each other, or a row past eight slices
+//
+// A row may start anywhere: the whole 16-byte packets inside it are handled as packets, the up to 2 * (kN - 1) elements
+// before and after them one per thread.
 __device__ int g_distill_status = 0;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -154,14 +164,251 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// 2^(from - to), 1 for equal references (two of -inf, two of +inf)
+__device__ __forceinline__ float rescale(float from, float to) { return from == to ? 1.0f : ex2(from - to); }
+
+// How the exponentials of the two softmaxes come about.
+enum ExpMode : int {
+  kOneExp = 0,    // no label term, or T = 1: one exponential serves both
+  kSquares = 1,   // T = 2 or 4: exp(x) is exp(x / T) squared once or twice
+  kTwoExps = 2,   // any other T
+};
+
+// What a row's softmaxes come down to, in every thread.
+struct RowStats {
+  float n, S, S1;   // reference and sum at temperature T, sum at 1 (its reference: T n where squared, else n1)
+  float n1;
+  float nt, St;     // teacher
+  bool some, known; // has a target, has a label
+  float kT, k1;     // factors of the two numerators in the gradient
+};
+
+template <int kMode>
+struct Exps {
+  float cT, c1;
+  int squarings;
+  __device__ __forceinline__ float numerator1(float v, float e, float n1) const {  // of the label term
+    if constexpr (kMode == kSquares) {
+      const float e2 = e * e;
+      return squarings == 2 ? e2 * e2 : e2;
+    }
+    if constexpr (kMode == kTwoExps) return ex2(fmaf(v, c1, -n1));
+    return e;
+  }
+  __device__ __forceinline__ void add(float v, float n, float n1, float& s, float& s1) const {
+    const float e = ex2(fmaf(v, cT, -n));
+    s += e;
+    if constexpr (kMode != kOneExp) s1 += numerator1(v, e, n1);
+  }
+  __device__ __forceinline__ float grad(float v, const RowStats& r) const {
+    const float e = ex2(fmaf(v, cT, -r.n));
+    if constexpr (kMode == kOneExp) return e * r.kT;  // kT holds both factors
+    return e * r.kT + numerator1(v, e, r.n1) * r.k1;
+  }
+};
+
+// An entry of a row's list (k < K) or its label (k = K): column or -1, teacher logit, own logit.
+template <typename T>
+__device__ __forceinline__ void load_entry(const DistillParams& p, bool hard, int64_t row, int k, int* col, float* t, float* zv) {
+  int id = -1;
+  *t = 0.0f;
+  *zv = 0.0f;
+  if (k < p.K) id = __ldg(p.ids + row * p.K + k);
+  else if (hard) id = __ldg(p.labels + row);
+  const bool ok = id >= 0 && id < p.C;
+  *col = ok ? id : -1;
+  if (ok) {
+    if (k < p.K) *t = teacher_at(p, row * p.K + k);
+    *zv = Cvt<T>::to_f(static_cast<const T*>(p.z)[row * p.ldz + id]);
+  }
+}
+// Running reference and sum of the teacher's weights.
+__device__ __forceinline__ void teacher_add(float t, float cT, float& nt, float& st) {
+  const float u = t * cT, to = fmaxf(nt, u);
+  const float ref = to == -INFINITY ? 0.0f : to;
+  st = st * (nt == -INFINITY ? 0.0f : rescale(nt, ref)) + ex2(u - ref);
+  nt = to;
+}
+__device__ __forceinline__ void finish_stats(const DistillParams& p, int mode, bool known, RowStats& r) {
+  if (r.S == 0.0f) r.S = r.S1 = __int_as_float(0x7fc00000);  // a row of -inf has no softmax
+  if (r.nt == -INFINITY) r.nt = 0.0f;
+  r.some = !(r.St == 0.0f);  // else no entries, or every entry has weight zero
+  r.known = known;
+  r.kT = r.some ? p.scale * (1.0f - p.alpha) * p.temperature / r.S : 0.0f;
+  r.k1 = known ? p.scale * p.alpha / r.S1 : 0.0f;
+  if (mode == kOneExp) r.kT += r.k1;
+}
+// The weight that entry j takes from the gradient at its column.
+__device__ __forceinline__ float entry_weight(const DistillParams& p, const RowStats& r, float cT, int j, float t) {
+  if (j == p.K) return p.scale * p.alpha;
+  return r.some ? p.scale * (1.0f - p.alpha) * p.temperature * (ex2(fmaf(t, cT, -r.nt)) / r.St) : 0.0f;
+}
+// p_k (log p_k - log q_k) without the sums' logarithms; natural logarithms
+__device__ __forceinline__ float cross_term(const RowStats& r, float cT, float t, float zv) {
+  constexpr float kLn2 = 0.6931471805599453f;
+  const float a = fmaf(t, cT, -r.nt), pk = ex2(a) / r.St;
+  return pk != 0.0f ? pk * (kLn2 * (a - fmaf(zv, cT, -r.n))) : 0.0f;
+}
+__device__ __forceinline__ float row_loss(const DistillParams& p, const RowStats& r, float cross, float z_label, float c1) {
+  constexpr float kLn2 = 0.6931471805599453f;
+  float loss = 0.0f;
+  if (r.some) loss = (1.0f - p.alpha) * p.temperature * p.temperature * (cross - logf(r.St) + logf(r.S));
+  if (r.known) loss += p.alpha * (logf(r.S1) - kLn2 * fmaf(z_label, c1, -r.n1));
+  return loss;
+}
+__device__ __forceinline__ float max_of(const Pack16<float>& v) { return fmaxf(fmaxf(v.v[0], v.v[1]), fmaxf(v.v[2], v.v[3])); }
+__device__ __forceinline__ float max_of(const Pack16<__nv_bfloat16>& v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__bfloat162float(m.x), __bfloat162float(m.y));
+}
+__device__ __forceinline__ float max_of(const Pack16<__half>& v) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__half2float(m.x), __half2float(m.y));
+}
+template <typename T>
+__device__ __forceinline__ int head_elements(const T* row, int64_t C) {
+  const int h = static_cast<int>(((16u - (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u)) & 15u) / sizeof(T));
+  return h < C ? h : static_cast<int>(C);
+}
+
+struct RowPlan {
+  int mode = 0, squarings = 0;
+  int packets = 0;   // warp kernel: packets per lane; 0 = block kernel
+  int threads = 0;   // block kernel
+  int ranks = 1;     // CTAs of a cluster per row
+  int slice = 0;     // packets per CTA (warp kernel: per row)
+  size_t smem = 0;
+};
+
+constexpr int kRowsPerBlock = 8;
+
+// One warp per row.
+template <typename T, int kPk, int kMode>
+__global__ void __launch_bounds__(32 * kRowsPerBlock) distill_warp_kernel(const DistillParams p, const RowPlan g) {
+  using PK = Pack16<T>;
+  constexpr int kN = PK::kN;
+  extern __shared__ __align__(16) uint8_t dsmem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int entries = p.K + 1;
+  const int words = (static_cast<int>(p.C) + 31) / 32;
+  // per warp: marks of columns, then the row's list with its label: column, teacher logit, own logit
+  uint32_t* bits_s = reinterpret_cast<uint32_t*>(dsmem) + warp * (words + 3 * entries);
+  int* col_s = reinterpret_cast<int*>(bits_s + words);
+  float* t_s = reinterpret_cast<float*>(col_s + entries);
+  float* z_s = t_s + entries;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + warp;
+  if (row >= p.B) return;  // whole warps: nothing below meets another warp
+  const bool hard = p.labels != nullptr && p.alpha > 0.0f;
+  const Exps<kMode> x{kLog2e / p.temperature, kLog2e, g.squarings};
+  const T* z = static_cast<const T*>(p.z) + row * p.ldz;
+  const int head = head_elements(z, p.C);
+  const int pn = (static_cast<int>(p.C) - head) / kN, tail0 = head + pn * kN;
+  const int edges = head + static_cast<int>(p.C) - tail0;
+  const int edge_col = lane < edges ? (lane < head ? lane : tail0 + lane - head) : -1;
+  const PK* packets = reinterpret_cast<const PK*>(z + head);
+  PK raw[kPk];
+#pragma unroll
+  for (int q = 0; q < kPk; ++q)
+    if (lane + 32 * q < pn) raw[q] = ld_stream(packets + lane + 32 * q);
+  const float fe = edge_col >= 0 ? Cvt<T>::to_f(z[edge_col]) : -INFINITY;
+  for (int i = lane; i < words; i += 32) bits_s[i] = 0u;
+  __syncwarp();
+  bool twice = false;
+  float nt = -INFINITY, st = 0.0f;
+  for (int k = lane; k < entries; k += 32) {
+    int col;
+    float t, zv;
+    load_entry<T>(p, hard, row, k, &col, &t, &zv);
+    col_s[k] = col;
+    t_s[k] = t;
+    z_s[k] = zv;
+    if (col >= 0) {
+      if (k < p.K) teacher_add(t, x.cT, nt, st);
+      if (p.dz && (atomicOr(bits_s + (col >> 5), 1u << (col & 31)) & (1u << (col & 31)))) twice = true;
+    }
+  }
+  float m = fe;
+#pragma unroll
+  for (int q = 0; q < kPk; ++q)
+    if (lane + 32 * q < pn) m = fmaxf(m, max_of(raw[q]));
+  m = warp_max(m);
+  RowStats r;
+  const float ref = m == -INFINITY ? 0.0f : m;
+  r.n = ref * x.cT;
+  r.n1 = kMode == kSquares ? r.n * p.temperature : ref * x.c1;
+  float s = 0.0f, s1 = 0.0f;
+#pragma unroll
+  for (int q = 0; q < kPk; ++q)
+    if (lane + 32 * q < pn) {
+      float f[kN];
+      unpack16(raw[q], f);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x.add(f[e], r.n, r.n1, s, s1);
+    }
+  if (edge_col >= 0) x.add(fe, r.n, r.n1, s, s1);
+  r.S = warp_sum(s);
+  r.S1 = kMode == kOneExp ? r.S : warp_sum(s1);
+  r.nt = warp_max(nt);
+  r.St = warp_sum(nt == -INFINITY ? st : st * rescale(nt, r.nt));
+  __syncwarp();
+  finish_stats(p, kMode, hard && col_s[p.K] >= 0, r);
+  if (r.some || r.known) {
+    float cross = 0.0f;
+    if (r.some) {
+      for (int k = lane; k < p.K; k += 32)
+        if (col_s[k] >= 0) cross += cross_term(r, x.cT, t_s[k], z_s[k]);
+      cross = warp_sum(cross);
+    }
+    if (lane == 0) p.loss[row] = row_loss(p, r, cross, z_s[p.K], x.c1);
+  } else if (lane == 0) {
+    p.loss[row] = 0.0f;
+  }
+  if (!p.dz) return;
+  T* out = static_cast<T*>(p.dz) + row * p.lddz;
+  PK* out_packets = reinterpret_cast<PK*>(out + head);
+  const bool dead = !r.some && !r.known;
+#pragma unroll
+  for (int q = 0; q < kPk; ++q)
+    if (lane + 32 * q < pn) {
+      float f[kN];
+      unpack16(raw[q], f);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) f[e] = x.grad(f[e], r);
+      if (dead) {
+#pragma unroll
+        for (int e = 0; e < kN; ++e) f[e] = 0.0f;
+      }
+      PK o;
+      pack16(o, f);
+      st_stream(out_packets + lane + 32 * q, o);
+    }
+  if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(dead ? 0.0f : x.grad(fe, r));
+  if (dead) return;
+  const bool dup = __any_sync(0xffffffffu, twice);
+  __syncwarp();  // the corrections come behind the row: other lanes, the same addresses
+  for (int k = lane; k < entries; k += 32) {
+    const int col = col_s[k];
+    if (col < 0) continue;
+    float w = 0.0f;
+    bool first = true;
+    if (dup) {
+      for (int j = 0; j < entries; ++j)
+        if (col_s[j] == col) {
+          if (j < k) first = false;
+          w += entry_weight(p, r, x.cT, j, t_s[j]);
+        }
+    } else {
+      w = entry_weight(p, r, x.cT, k, t_s[k]);
+    }
+    if (first) out[col] = Cvt<T>::from_f(x.grad(z_s[k], r) - w);
+  }
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
 __device__ __forceinline__ uint32_t cluster_index() {
@@ -186,91 +433,42 @@ __device__ __forceinline__ void st_peer_shared(const float* local, uint32_t rank
 
 constexpr int kRowThreads = 512;
 constexpr int kMaxRanks = 8;
+constexpr int kRowCtas = 3;   // CTAs per SM that the block kernel is sized for: while one waits for its row, others work
 
-// How the exponentials of the two softmaxes come about.
-enum ExpMode : int {
-  kOneExp = 0,    // no label term, or T = 1: one exponential serves both
-  kSquares = 1,   // T = 2 or 4: exp(x) is exp(x / T) squared once or twice
-  kTwoExps = 2,   // any other T: the logits stay in registers and both are taken again when the gradient is written
-};
-
-struct RowPlan {
-  int mode = 0;
-  int squarings = 0;
-  int threads = 0, packets = 0;  // packets of 16 bytes per thread
-  int ranks = 1;                 // CTAs (of a cluster) per row
-  int slice = 0;                 // packets per CTA
-  size_t smem = 0;
-  int early = 0;                 // one CTA per SM: request the next row before any arithmetic
-};
-
-// A running maximum and the sum of exponentials below it.
-__device__ __forceinline__ float rescale(float m, float to, float c) { return m == to ? 1.0f : ex2((m - to) * c); }
-
-// One row per CTA, or per cluster with a contiguous slice for each CTA. The slice sits in registers; the next row's is
-// on its way to shared memory meanwhile. A row may start anywhere: the whole 16-byte packets inside it are copied and kept as
-// packets, and the up to 2 * (kN - 1) elements before and after them by one thread each of rank 0.
-//
-// Each thread takes its exponentials below its own maximum, so a row needs one reduction (and in a cluster one barrier)
-// for maximum and sum together; the thread's factor to the row's maximum joins the normalisation.
-template <typename T, int kPk, int kMode>
-__global__ void __launch_bounds__(kRowThreads) distill_row_kernel(const DistillParams p, const RowPlan g) {
+template <typename T, int kMode>
+__global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(const DistillParams p, const RowPlan g) {
   using PK = Pack16<T>;
   constexpr int kN = PK::kN;
   extern __shared__ __align__(16) uint8_t dsmem[];
-  // [slice][mbarrier 16 B][bitmap x 2][entries x 2: column, teacher logit, own logit]
-  const int bits_words = (g.slice * kN + 2 * kN + 31) / 32;
-  const int entries = p.K + 1;  // the row's list, then its label
+  // [slice][mbarrier 16 B][marks x 2][entries x 2: column, teacher logit, own logit]; rows alternate between the two
+  const int words = (g.slice * kN + 2 * kN + 31) / 32;
+  const int entries = p.K + 1;
   const PK* row_s = reinterpret_cast<const PK*>(dsmem);
   uint32_t* bits_s = reinterpret_cast<uint32_t*>(dsmem + static_cast<size_t>(g.slice) * 16 + 16);
-  int* col_s = reinterpret_cast<int*>(bits_s + 2 * bits_words);
-  float* t_s = reinterpret_cast<float*>(col_s + 2 * entries);
-  float* z_s = t_s + 2 * entries;
+  int* col_all = reinterpret_cast<int*>(bits_s + 2 * words);
   __shared__ float red[2][5][kRowThreads / 32];
   __shared__ float peer[2][kMaxRanks][3];
   __shared__ int twice[2];    // some column occurs more than once
   __shared__ int wait_failed;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x, nwarps = nthreads >> 5;
-  const uint32_t nranks = g.ranks > 1 ? cluster_size() : 1, rank = g.ranks > 1 ? cluster_rank() : 0;
+  const uint32_t rank = g.ranks > 1 ? cluster_rank() : 0;
   const int64_t first_row = g.ranks > 1 ? cluster_index() : blockIdx.x, row_step = g.ranks > 1 ? cluster_count() : gridDim.x;
   const uint32_t buf = sm100::smem_addr(dsmem), bar = buf + static_cast<uint32_t>(g.slice) * 16;
-  const T* z = static_cast<const T*>(p.z);
-  T* dz = static_cast<T*>(p.dz);
   const bool hard = p.labels != nullptr && p.alpha > 0.0f;
-  const float cT = kLog2e / p.temperature, c1 = kLog2e;
-  const float wT = p.scale * (1.0f - p.alpha) * p.temperature, w1 = p.scale * p.alpha;
+  const Exps<kMode> x{kLog2e / p.temperature, kLog2e, g.squarings};
   const int p0 = static_cast<int>(rank) * g.slice;
+  const int C = static_cast<int>(p.C);
 
-  // elements before the first whole packet of a row, and packets of this CTA
-  auto head_of = [&](int64_t row) {
-    const uint32_t a = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(z + row * p.ldz)) & 15u;
-    const int h = static_cast<int>(((16u - a) & 15u) / sizeof(T));
-    return h < p.C ? h : static_cast<int>(p.C);
-  };
   auto packets_of = [&](int head) {
-    const int n = static_cast<int>((p.C - head) / kN) - p0;
+    const int n = (C - head) / kN - p0;
     return n < 0 ? 0 : n < g.slice ? n : g.slice;
   };
-  bool piped = true;  // false once a copy did not arrive: the rest of the rows runs on what the buffer holds
   auto fetch = [&](int64_t row) {  // thread 0
-    const int head = head_of(row), n = packets_of(head);
+    const T* z = static_cast<const T*>(p.z) + row * p.ldz;
+    const int head = head_elements(z, p.C), n = packets_of(head);
     if (n > 0) {
       sm100::mbar_expect_tx(bar, static_cast<uint32_t>(n) * 16);
-      sm100::bulk_copy_g2s(buf, z + row * p.ldz + head + static_cast<int64_t>(p0) * kN, static_cast<uint32_t>(n) * 16, bar);
-    }
-  };
-  // an entry of a row's list (k < K) or its label (k = K)
-  auto entry = [&](int64_t row, int k, int* col, float* t, float* zv) {
-    int id = -1;
-    *t = 0.0f;
-    *zv = 0.0f;
-    if (k < p.K) id = __ldg(p.ids + row * p.K + k);
-    else if (hard) id = __ldg(p.labels + row);
-    const bool ok = id >= 0 && id < p.C;
-    *col = ok ? id : -1;
-    if (ok) {
-      if (k < p.K) *t = teacher_at(p, row * p.K + k);
-      *zv = Cvt<T>::to_f(z[row * p.ldz + id]);
+      sm100::bulk_copy_g2s(buf, z + head + static_cast<int64_t>(p0) * kN, static_cast<uint32_t>(n) * 16, bar);
     }
   };
 
@@ -280,241 +478,173 @@ __global__ void __launch_bounds__(kRowThreads) distill_row_kernel(const DistillP
     wait_failed = 0;
     twice[0] = twice[1] = 0;
   }
-  for (int i = tid; i < 2 * bits_words; i += nthreads) bits_s[i] = 0u;
+  for (int i = tid; i < 2 * words; i += nthreads) bits_s[i] = 0u;
   __syncthreads();
-  int my_col = -1;
-  float my_t = 0.0f, my_z = 0.0f;  // entry `tid` of the row at hand, read one row ahead
-  if (first_row < p.B) {
-    if (tid == 0) fetch(first_row);
-    if (tid < entries) entry(first_row, tid, &my_col, &my_t, &my_z);
-  }
+  if (tid == 0 && first_row < p.B) fetch(first_row);
+  bool piped = true;  // false once a copy did not arrive: the remaining rows run on what the buffer holds
   uint32_t phase = 0;
   int par = 0;
   for (int64_t row = first_row; row < p.B; row += row_step, par ^= 1) {
-    const int head = head_of(row), pn = packets_of(head);
-    const int64_t next = row + row_step;
-    // the edges: elements [0, head) and [tail0, C), one per thread of rank 0
-    const int tail0 = head + static_cast<int>((p.C - head) / kN) * kN;
-    const int edges = rank == 0 ? head + static_cast<int>(p.C) - tail0 : 0;
+    const T* z = static_cast<const T*>(p.z) + row * p.ldz;
+    const int head = head_elements(z, p.C), pn = packets_of(head);
+    const int tail0 = head + (C - head) / kN * kN;
+    const int edges = rank == 0 ? head + C - tail0 : 0;  // rank 0 has the elements outside the packets
     const int edge_col = tid < edges ? (tid < head ? tid : tail0 + tid - head) : -1;
-    float fe = edge_col >= 0 ? Cvt<T>::to_f(z[row * p.ldz + edge_col]) : -INFINITY;
+    const float fe = edge_col >= 0 ? Cvt<T>::to_f(z[edge_col]) : -INFINITY;
+    uint32_t* bits = bits_s + par * words;
+    int* col_s = col_all + par * 3 * entries;
+    float* t_s = reinterpret_cast<float*>(col_s + entries);
+    float* z_s = t_s + entries;
+    // the place of a column in this CTA's marks, -1 for another CTA's column
+    auto place = [&](int col) {
+      if (col < head) return rank == 0 ? g.slice * kN + col : -1;
+      if (col >= tail0) return rank == 0 ? g.slice * kN + kN + col - tail0 : -1;
+      const int at = col - head - p0 * kN;
+      return at >= 0 && at < pn * kN ? at : -1;
+    };
+    // the row's list, while the row itself is on its way
+    float nt = -INFINITY, st = 0.0f;
+    for (int k = tid; k < entries; k += nthreads) {
+      int col;
+      float t, zv;
+      load_entry<T>(p, hard, row, k, &col, &t, &zv);
+      col_s[k] = col;
+      t_s[k] = t;
+      z_s[k] = zv;
+      if (col >= 0) {
+        if (k < p.K) teacher_add(t, x.cT, nt, st);
+        const int at = p.dz ? place(col) : -1;
+        if (at >= 0 && (atomicOr(bits + (at >> 5), 1u << (at & 31)) & (1u << (at & 31)))) twice[par] = 1;
+      }
+    }
     if (pn > 0 && piped) {
       if (!sm100::mbar_wait_bounded(bar, phase, rowk::kRowWaitBudgetNs)) wait_failed = 1;
       phase ^= 1u;
     }
-    float f[kPk][kN];
-#pragma unroll
-    for (int q = 0; q < kPk; ++q) {
-      const int pi = tid + q * nthreads;
-      if (pi < pn) {
-        unpack16(row_s[pi], f[q]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kN; ++e) f[q][e] = -INFINITY;
-      }
-    }
-    auto refill = [&]() {  // behind a barrier: everybody holds its packets
-      if (wait_failed) piped = false;
-      if (tid == 0 && next < p.B && piped) {
-        sm100::fence_generic_to_async_smem();
-        fetch(next);
-      }
-    };
-    if (g.early) {
-      __syncthreads();
-      refill();
-    }
     float m = fe;
-#pragma unroll
-    for (int q = 0; q < kPk; ++q)
-#pragma unroll
-      for (int e = 0; e < kN; ++e) m = fmaxf(m, f[q][e]);
-    // the row's list: staged for everybody, its columns marked, the teacher's sum
-    float mt = -INFINITY, st = 0.0f;
-    for (int k = tid; k < entries; k += nthreads) {
-      if (k != tid) entry(row, k, &my_col, &my_t, &my_z);
-      col_s[par * entries + k] = my_col;
-      t_s[par * entries + k] = my_t;
-      z_s[par * entries + k] = my_z;
-      if (my_col >= 0) {
-        if (k < p.K) {
-          const float to = fmaxf(mt, my_t), ref = to == -INFINITY ? 0.0f : to;
-          st = st * (mt == -INFINITY ? 0.0f : rescale(mt, ref, cT)) + ex2((my_t - ref) * cT);
-          mt = to;
-        }
-        if (p.dz) {
-          const int at = my_col < head || my_col >= tail0 ? -1 : my_col - head - p0 * kN;
-          const bool mine = at >= 0 ? at < pn * kN : at == -1 && rank == 0 && (my_col < head || my_col >= tail0);
-          if (mine) {
-            const int bit = at >= 0 ? at : g.slice * kN + (my_col < head ? my_col : kN + my_col - tail0);
-            if (atomicOr(bits_s + par * bits_words + (bit >> 5), 1u << (bit & 31)) & (1u << (bit & 31))) twice[par] = 1;
-          }
-        }
-      }
-    }
-    // exponentials below the thread's own maximum
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f, s1 = 0.0f;
-    auto both = [&](float& v) {  // v: logit -> exponential (kTwoExps: stays a logit)
-      const float d = v - ref;
-      const float e = ex2(d * cT);
-      s += e;
-      if constexpr (kMode == kSquares) {
-        const float e2 = e * e;
-        s1 += g.squarings == 2 ? e2 * e2 : e2;
-      }
-      if constexpr (kMode == kTwoExps) s1 += ex2(d * c1);
-      else v = e;
-    };
-#pragma unroll
-    for (int q = 0; q < kPk; ++q)
-#pragma unroll
-      for (int e = 0; e < kN; ++e) both(f[q][e]);
-    both(fe);
+#pragma unroll 4
+    for (int pi = tid; pi < pn; pi += nthreads) m = fmaxf(m, max_of(row_s[pi]));
+    m = warp_max(m);
+    RowStats r;
     {
-      const float mw = warp_max(m), mtw = warp_max(mt);
-      const float k = m == -INFINITY ? (s != s ? s : 0.0f) : rescale(m, mw, cT);
-      s = warp_sum(s * k);
-      if constexpr (kMode != kOneExp) s1 = warp_sum(s1 * (m == -INFINITY ? 0.0f : rescale(m, mw, c1)));
-      st = warp_sum(mt == -INFINITY ? st : st * rescale(mt, mtw, cT));
+      const float ref = m == -INFINITY ? 0.0f : m;
+      const float n = ref * x.cT, n1 = kMode == kSquares ? n * p.temperature : ref * x.c1;
+      float s = 0.0f, s1 = 0.0f;
+#pragma unroll 2
+      for (int pi = tid; pi < pn; pi += nthreads) {
+        float f[kN];
+        unpack16(row_s[pi], f);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) x.add(f[e], n, n1, s, s1);
+      }
+      if (edge_col >= 0) x.add(fe, n, n1, s, s1);
+      s = warp_sum(s);
+      if constexpr (kMode != kOneExp) s1 = warp_sum(s1);
+      const float ntw = warp_max(nt);
+      st = warp_sum(nt == -INFINITY ? st : st * rescale(nt, ntw));
       if (lane == 0) {
-        red[par][0][warp] = mw;
+        red[par][0][warp] = m;
         red[par][1][warp] = s;
         red[par][2][warp] = s1;
-        red[par][3][warp] = mtw;
+        red[par][3][warp] = ntw;
         red[par][4][warp] = st;
       }
     }
     __syncthreads();
-    if (!g.early) refill();
-    float M, S, S1, Mt, St;
     {
+      // every warp folds the warps' parts for itself, in the same order
       const bool in = lane < nwarps;
       const float a = in ? red[par][0][lane] : -INFINITY, at = in ? red[par][3][lane] : -INFINITY;
-      M = warp_max(a);
-      Mt = warp_max(at);
-      S = warp_sum(in ? red[par][1][lane] * (a == -INFINITY ? 1.0f : rescale(a, M, cT)) : 0.0f);
-      S1 = kMode == kOneExp ? S : warp_sum(in ? red[par][2][lane] * (a == -INFINITY ? 1.0f : rescale(a, M, c1)) : 0.0f);
-      St = warp_sum(in ? red[par][4][lane] * (at == -INFINITY ? 1.0f : rescale(at, Mt, cT)) : 0.0f);
+      m = warp_max(a);
+      r.nt = warp_max(at);
+      r.S = warp_sum(in ? red[par][1][lane] * (a == m ? 1.0f : ex2(__fmul_rn(a, x.cT) - __fmul_rn(m, x.cT))) : 0.0f);
+      r.S1 = kMode == kOneExp ? r.S : warp_sum(in ? red[par][2][lane] * (a == m ? 1.0f : ex2(__fmul_rn(a, x.c1) - __fmul_rn(m, x.c1))) : 0.0f);
+      r.St = warp_sum(in ? red[par][4][lane] * rescale(at, r.nt) : 0.0f);
     }
-    if (nranks > 1) {
-      if (warp == 0 && lane < static_cast<int>(nranks)) {
-        st_peer_shared(&peer[par][rank][0], lane, M);
-        st_peer_shared(&peer[par][rank][1], lane, S);
-        st_peer_shared(&peer[par][rank][2], lane, S1);
+    if (g.ranks > 1) {
+      if (warp == 0 && lane < g.ranks) {
+        st_peer_shared(&peer[par][rank][0], lane, m);
+        st_peer_shared(&peer[par][rank][1], lane, r.S);
+        st_peer_shared(&peer[par][rank][2], lane, r.S1);
       }
       __syncwarp();
       cluster_barrier();  // the other parity's slots are rewritten behind this row's barrier only
-      float a = -INFINITY, b = 0.0f, c = 0.0f;
-      for (uint32_t r = 0; r < nranks; ++r) a = fmaxf(a, peer[par][r][0]);
-      for (uint32_t r = 0; r < nranks; ++r) {
-        const float pm = peer[par][r][0];
-        b += peer[par][r][1] * (pm == -INFINITY ? 1.0f : rescale(pm, a, cT));
-        c += peer[par][r][2] * (pm == -INFINITY ? 1.0f : rescale(pm, a, c1));
+      float a = -INFINITY;
+      for (int k = 0; k < g.ranks; ++k) a = fmaxf(a, peer[par][k][0]);
+      r.S = r.S1 = 0.0f;
+      for (int k = 0; k < g.ranks; ++k) {
+        const float pm = peer[par][k][0];
+        r.S += peer[par][k][1] * (pm == a ? 1.0f : ex2(__fmul_rn(pm, x.cT) - __fmul_rn(a, x.cT)));
+        r.S1 += peer[par][k][2] * (pm == a ? 1.0f : ex2(__fmul_rn(pm, x.c1) - __fmul_rn(a, x.c1)));
       }
-      M = a, S = b, S1 = kMode == kOneExp ? b : c;
+      m = a;
+      if constexpr (kMode == kOneExp) r.S1 = r.S;
     }
-    if (M == -INFINITY && !(S != S)) S = S1 = __int_as_float(0x7fc00000);  // a row of -inf has no softmax
-    if (Mt == -INFINITY) Mt = 0.0f;
-    const bool some = !(St == 0.0f);  // no entries, or every entry has weight zero: no target
-    const bool known = hard && col_s[par * entries + p.K] >= 0;
-    const float kT = some ? wT / S : 0.0f, k1 = known ? w1 / S1 : 0.0f;
-    // the next row's entries: their loads run while this row is written
-    int next_col = -1;
-    float next_t = 0.0f, next_z = 0.0f;
-    if (next < p.B && tid < entries) entry(next, tid, &next_col, &next_t, &next_z);
-
-    if (rank == 0 && warp == 0) {
-      const float invT = 1.0f / p.temperature;
-      float cross = 0.0f;
-      if (some) {
-        for (int k = lane; k < p.K; k += 32) {
-          if (col_s[par * entries + k] < 0) continue;
-          const float a = (t_s[par * entries + k] - Mt) * invT;
-          const float pk = ex2((t_s[par * entries + k] - Mt) * cT) / St;
-          if (pk != 0.0f) cross += pk * (a - (z_s[par * entries + k] - M) * invT);
+    {
+      const float ref = m == -INFINITY ? 0.0f : m;
+      r.n = ref * x.cT;
+      r.n1 = kMode == kSquares ? r.n * p.temperature : ref * x.c1;
+    }
+    finish_stats(p, kMode, hard && col_s[p.K] >= 0, r);
+    const bool dead = !r.some && !r.known;
+    T* out = static_cast<T*>(p.dz) + row * p.lddz;
+    if (p.dz) {
+      PK* packets = reinterpret_cast<PK*>(out + head) + p0;
+#pragma unroll 2
+      for (int pi = tid; pi < pn; pi += nthreads) {
+        float f[kN];
+        unpack16(row_s[pi], f);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) f[e] = x.grad(f[e], r);
+        if (dead) {
+#pragma unroll
+          for (int e = 0; e < kN; ++e) f[e] = 0.0f;
         }
+        PK o;
+        pack16(o, f);
+        st_stream(packets + pi, o);
+      }
+      if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(dead ? 0.0f : x.grad(fe, r));
+      if (tid == 0) twice[par ^ 1] = 0;  // last read one row ago, next set behind this barrier
+    }
+    __syncthreads();  // the buffer is free; the corrections below come behind the row's stores
+    if (wait_failed) piped = false;
+    if (tid == 0 && row + row_step < p.B && piped) {
+      sm100::fence_generic_to_async_smem();
+      fetch(row + row_step);
+    }
+    if (rank == 0 && warp == nwarps - 1) {
+      float cross = 0.0f;
+      if (r.some) {
+        for (int k = lane; k < p.K; k += 32)
+          if (col_s[k] >= 0) cross += cross_term(r, x.cT, t_s[k], z_s[k]);
         cross = warp_sum(cross);
       }
-      if (lane == 0) {
-        float loss = 0.0f;
-        if (some) loss = (1.0f - p.alpha) * p.temperature * p.temperature * (cross - logf(St) + logf(S));
-        if (known) loss += p.alpha * (logf(S1) + M - z_s[par * entries + p.K]);
-        p.loss[row] = loss;
-      }
+      if (lane == 0) p.loss[row] = row_loss(p, r, cross, z_s[p.K], x.c1);
     }
     if (p.dz) {
-      T* out = dz + row * p.lddz;
-      PK* packets = reinterpret_cast<PK*>(out + head) + p0;
-      const bool dead = !some && !known;
-      const float up = m == -INFINITY ? 0.0f : rescale(m, M, cT);
-      const float gT = kMode == kOneExp ? up * (kT + k1) : up * kT;
-      const float g1 = kMode == kSquares ? (m == -INFINITY ? 0.0f : rescale(m, M, c1)) * k1 : 0.0f;
-      auto grad = [&](float v) {
-        if constexpr (kMode == kOneExp) return v * gT;
-        if constexpr (kMode == kSquares) {
-          const float v2 = v * v;
-          return v * gT + (g.squarings == 2 ? v2 * v2 : v2) * g1;
-        }
-        const float d = v - M;
-        return ex2(d * cT) * kT + ex2(d * c1) * k1;
-      };
-#pragma unroll
-      for (int q = 0; q < kPk; ++q) {
-        const int pi = tid + q * nthreads;
-        if (pi < pn) {
-          PK o;
-          float v[kN];
-#pragma unroll
-          for (int e = 0; e < kN; ++e) v[e] = dead ? 0.0f : grad(f[q][e]);
-          pack16(o, v);
-          st_stream(packets + pi, o);
-        }
-      }
-      if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(dead ? 0.0f : grad(fe));
-      if (tid == 0) twice[par ^ 1] = 0;  // last read one row ago, next set behind this barrier
-      __syncthreads();  // the corrections come behind the row: other threads, the same addresses
-      if (!dead) {
-        const bool dup = twice[par] != 0;
-        for (int k = tid; k < entries; k += nthreads) {
-          const int col = col_s[par * entries + k];
-          if (col < 0) continue;
-          const bool edge = col < head || col >= tail0;
-          const int at = col - head - p0 * kN;
-          if (edge ? rank != 0 : (at < 0 || at >= pn * kN)) continue;
-          auto weight = [&](int j) {
-            return j == p.K ? w1 : some ? wT * (ex2((t_s[par * entries + j] - Mt) * cT) / St) : 0.0f;
-          };
-          float w = 0.0f;
-          bool first = true;
-          if (dup) {
-            for (int j = 0; j < entries; ++j)
-              if (col_s[par * entries + j] == col) {
-                if (j < k) first = false;
-                w += weight(j);
-              }
-          } else {
-            w = weight(k);
-          }
-          if (!first) continue;
-          const float d = z_s[par * entries + k] - M;
-          out[col] = Cvt<T>::from_f(ex2(d * cT) * kT + (k1 != 0.0f ? ex2(d * c1) * k1 : 0.0f) - w);
-        }
-      }
-      // this row's marks
+      const bool dup = twice[par] != 0;
       for (int k = tid; k < entries; k += nthreads) {
-        const int col = col_s[par * entries + k];
-        if (col < 0) continue;
-        const bool edge = col < head || col >= tail0;
-        const int at = col - head - p0 * kN;
-        if (edge ? rank != 0 : (at < 0 || at >= pn * kN)) continue;
-        const int bit = !edge ? at : g.slice * kN + (col < head ? col : kN + col - tail0);
-        bits_s[par * bits_words + (bit >> 5)] = 0u;
+        const int col = col_s[k];
+        const int at = col >= 0 ? place(col) : -1;
+        if (at < 0) continue;
+        bits[at >> 5] = 0u;  // this row's marks go
+        float w = 0.0f;
+        bool first = !dead;
+        if (dup) {
+          for (int j = 0; j < entries; ++j)
+            if (col_s[j] == col) {
+              if (j < k) first = false;
+              w += entry_weight(p, r, x.cT, j, t_s[j]);
+            }
+        } else {
+          w = entry_weight(p, r, x.cT, k, t_s[k]);
+        }
+        if (first) out[col] = Cvt<T>::from_f(x.grad(z_s[k], r) - w);
       }
     }
-    my_col = next_col, my_t = next_t, my_z = next_z;
   }
-  if (nranks > 1) cluster_barrier();  // nobody leaves while a peer may still write its shared memory
+  if (g.ranks > 1) cluster_barrier();  // nobody leaves while a peer may still write its shared memory
   if (wait_failed) {
     if (tid == 0) atomicExch(&g_distill_status, 1);
     for (int i = 0; i < 64; ++i) __nanosleep(16384);  // error path only: let a late copy land
@@ -524,7 +654,6 @@ __global__ void __launch_bounds__(kRowThreads) distill_row_kernel(const DistillP
 template <typename T>
 bool plan_rows(const DistillParams& p, RowPlan* out) {
   constexpr int kN = Pack16<T>::kN;
-  constexpr int kMaxPk = 64 / kN;
   RowPlan g;
   if (!aligned_to(p.z, sizeof(T)) || (p.dz && !aligned_to(p.dz, sizeof(T)))) return false;
   if (p.dz) {  // packets of z and dz have to start at the same places in every row
@@ -535,56 +664,52 @@ bool plan_rows(const DistillParams& p, RowPlan* out) {
   g.mode = !hard || p.temperature == 1.0f ? kOneExp : p.temperature == 2.0f || p.temperature == 4.0f ? kSquares : kTwoExps;
   g.squarings = p.temperature == 4.0f ? 2 : 1;
   const int64_t packets = p.C / kN > 0 ? p.C / kN : 1;
-  g.ranks = 1;
-  while (g.ranks < kMaxRanks && (packets + g.ranks - 1) / g.ranks > static_cast<int64_t>(kRowThreads) * kMaxPk) g.ranks *= 2;
-  if (const char* e = std::getenv("AICF_DISTILL_RANKS")) { const int v = std::atoi(e); if (v > g.ranks) g.ranks = v; }
+  const size_t list = static_cast<size_t>(p.K + 1) * 12;
+  if (p.C <= 2048) {
+    const int per = static_cast<int>((packets + 31) / 32);
+    g.packets = 1;
+    while (g.packets < per) g.packets *= 2;
+    g.slice = static_cast<int>(packets);
+    g.smem = kRowsPerBlock * (static_cast<size_t>((p.C + 31) / 32) * 4 + list);
+    *out = g;
+    return true;
+  }
+  auto bytes = [&](int64_t slice) {
+    return static_cast<size_t>(slice) * 16 + 16 + 2 * static_cast<size_t>((slice * kN + 2 * kN + 31) / 32) * 4 + 2 * list;
+  };
+  constexpr size_t kShare = (227 * 1024) / kRowCtas - 2048;  // an SM's shared memory over its CTAs, less the static part
+  int limit_ranks = kMaxRanks;
+  while (g.ranks < limit_ranks && bytes((packets + g.ranks - 1) / g.ranks) > kShare) g.ranks *= 2;
+  if (const char* e = std::getenv("AICF_DISTILL_RANKS")) { const int v = std::atoi(e); if (v > 0) g.ranks = v; }
   const int64_t slice = (packets + g.ranks - 1) / g.ranks;
-  if (slice > static_cast<int64_t>(kRowThreads) * kMaxPk) return false;
-  g.slice = static_cast<int>(slice);
-  int grow = 32 / kN; 
-  if (const char* e = std::getenv("AICF_DISTILL_GROW")) grow = std::atoi(e);
-  g.threads = 32;
-  while (g.threads < kRowThreads && static_cast<int64_t>(g.threads) * grow < slice) g.threads *= 2;
-  const int per = static_cast<int>((slice + g.threads - 1) / g.threads);
-  g.packets = 1;
-  while (g.packets < per) g.packets *= 2;
-  const size_t words = (slice * kN + 2 * kN + 31) / 32;
-  g.smem = static_cast<size_t>(slice) * 16 + 16 + 2 * words * 4 + 2 * static_cast<size_t>(p.K + 1) * 12;
+  g.smem = bytes(slice);
   if (g.smem > 200 * 1024) return false;
+  g.slice = static_cast<int>(slice);
+  int grow = 4; 
+  if (const char* e = std::getenv("AICF_DISTILL_GROW")) grow = std::atoi(e);
+  g.threads = 128;
+  while (g.threads < kRowThreads && static_cast<int64_t>(g.threads) * grow < slice) g.threads *= 2;
   *out = g;
   return true;
 }
 
-template <typename T, int kPk, int kMode>
-Status launch_rows(const DistillParams& p, RowPlan g, cudaStream_t stream) {
-  auto kernel = distill_row_kernel<T, kPk, kMode>;
+template <typename T, int kMode>
+Status launch_block_rows(const DistillParams& p, const RowPlan& g, cudaStream_t stream) {
+  auto kernel = distill_block_kernel<T, kMode>;
   static PerDeviceOnce opt_in;
   if (!opt_in.run([&] { return rowk::allow_smem(kernel, 200 * 1024); })) {
     cudaGetLastError();
     return Status::Internal;
   }
-  // resident blocks per SM, by threads, registers (allocated to warps in units of 256) and shared memory
-  static std::atomic<int> kernel_regs{0};
-  int regs = kernel_regs.load(std::memory_order_relaxed);
-  if (regs == 0) {
-    cudaFuncAttributes a{};
-    if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess) {
-      cudaGetLastError();
-      return Status::Internal;
-    }
-    regs = a.numRegs;
-    kernel_regs.store(regs, std::memory_order_relaxed);
-  }
-  const int by_regs = 65536 / (((regs + 7) / 8 * 8) * g.threads);
-  int resident = rowk::row_pipe_blocks_per_sm(g.threads, g.smem + 1024);
-  if (resident > by_regs) resident = by_regs > 0 ? by_regs : 1;
-  g.early = resident == 1;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(g.ranks);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  // registers allow kRowCtas blocks of kRowThreads threads
+  int resident = rowk::row_pipe_blocks_per_sm(g.threads, g.smem + 1024);
+  if (resident > kRowCtas * kRowThreads / g.threads) resident = kRowCtas * kRowThreads / g.threads;
   int over = 1;
   if (const char* e = std::getenv("AICF_DISTILL_OVER")) over = std::atoi(e);
   const int64_t slots = static_cast<int64_t>(sm_count()) * resident * over / g.ranks;
@@ -601,23 +726,37 @@ Status launch_rows(const DistillParams& p, RowPlan g, cudaStream_t stream) {
   }
   return launch_status();
 }
-template <typename T, int kPk>
+template <typename T, int kPk, int kMode>
+Status launch_warp_rows(const DistillParams& p, const RowPlan& g, cudaStream_t stream) {
+  auto kernel = distill_warp_kernel<T, kPk, kMode>;
+  static PerDeviceOnce opt_in;
+  if (!opt_in.run([&] { return rowk::allow_smem(kernel, 110 * 1024); })) {
+    cudaGetLastError();
+    return Status::Internal;
+  }
+  const int64_t blocks = (p.B + kRowsPerBlock - 1) / kRowsPerBlock;
+  if (blocks > 0x7fffffff) return Status::InvalidArgument;
+  kernel<<<static_cast<unsigned>(blocks), 32 * kRowsPerBlock, g.smem, stream>>>(p, g);
+  return launch_status();
+}
+template <typename T, int kMode>
 Status launch_mode(const DistillParams& p, const RowPlan& g, cudaStream_t stream) {
-  if (g.mode == kOneExp) return launch_rows<T, kPk, kOneExp>(p, g, stream);
-  if (g.mode == kSquares) return launch_rows<T, kPk, kSquares>(p, g, stream);
-  return launch_rows<T, kPk, kTwoExps>(p, g, stream);
+  switch (g.packets) {
+    case 0: return launch_block_rows<T, kMode>(p, g, stream);
+    case 1: return launch_warp_rows<T, 1, kMode>(p, g, stream);
+    case 2: return launch_warp_rows<T, 2, kMode>(p, g, stream);
+    case 4: return launch_warp_rows<T, 4, kMode>(p, g, stream);
+    case 8: return launch_warp_rows<T, 8, kMode>(p, g, stream);
+    default: break;
+  }
+  if constexpr (sizeof(T) == 4) return launch_warp_rows<T, 16, kMode>(p, g, stream);
+  return Status::Internal;
 }
 template <typename T>
 Status run_rows(const DistillParams& p, const RowPlan& g, cudaStream_t stream) {
-  switch (g.packets) {
-    case 1: return launch_mode<T, 1>(p, g, stream);
-    case 2: return launch_mode<T, 2>(p, g, stream);
-    case 4: return launch_mode<T, 4>(p, g, stream);
-    case 8: return launch_mode<T, 8>(p, g, stream);
-    default: break;
-  }
-  if constexpr (sizeof(T) == 4) return launch_mode<T, 16>(p, g, stream);
-  return Status::Internal;
+  if (g.mode == kOneExp) return launch_mode<T, kOneExp>(p, g, stream);
+  if (g.mode == kSquares) return launch_mode<T, kSquares>(p, g, stream);
+  return launch_mode<T, kTwoExps>(p, g, stream);
 }
 
 bool rows_ok(const TensorDesc& t, int64_t B, int64_t C) {
