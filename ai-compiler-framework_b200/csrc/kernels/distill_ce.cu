@@ -14,7 +14,10 @@
 // A row without entries has no distillation term, a row whose label lies outside [0,C) no label term (zero loss and zero
 // gradient both times). The same column may stand in a row's list more than once. loss_row carries no `scale`.
 // A row without either term gets zeros whatever its logits hold. dz may be z itself; otherwise outputs do not overlap inputs.
+#include <array>
 #include <cstdlib>
+#include <map>
+#include <mutex>
 
 #include "row_pipeline.cuh"
 
@@ -183,29 +186,115 @@ struct RowStats {
   float kT, k1;     // factors of the two numerators in the gradient
 };
 
+// Pairs of fp32 values: one instruction for two, which is what the 16-bit rows need (they are bound by issue).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t v) {
+  const float2 u = split(v);
+  return pair(ex2(u.x), ex2(u.y));
+}
+// 2^u for u <= 0 on the FMA pipe: u = i + f with i the nearest integer, 2^f by its Taylor polynomial of degree 6 (|f| <= 1/2:
+// off by at most (ln2 / 2)^7 / 7! = 1.2e-7), i added to the exponent. Below 2^-126 the result is 0; a NaN stays one. Rows with
+// two exponentials per logit take one of them here, because the special-function unit serves four lanes per clock and
+// scheduler only.
+__device__ __forceinline__ uint64_t ex2_pair_fma(uint64_t v) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the integer lands in the low mantissa bits
+  const float2 u = split(v);
+  const uint64_t t = add2(v, pair(kMagic, kMagic));
+  const uint64_t f = add2(v, mul2(add2(t, pair(-kMagic, -kMagic)), pair(-1.0f, -1.0f)));
+  uint64_t q = pair(1.54035303933816e-4f, 1.54035303933816e-4f);                        // ln2^6 / 6!
+  q = fma2(q, f, pair(1.33335581464284e-3f, 1.33335581464284e-3f));                     // ln2^5 / 5!
+  q = fma2(q, f, pair(9.61812910762848e-3f, 9.61812910762848e-3f));                     // ln2^4 / 4!
+  q = fma2(q, f, pair(5.55041086648216e-2f, 5.55041086648216e-2f));                     // ln2^3 / 3!
+  q = fma2(q, f, pair(2.40226506959101e-1f, 2.40226506959101e-1f));                     // ln2^2 / 2
+  q = fma2(q, f, pair(6.93147180559945e-1f, 6.93147180559945e-1f));                     // ln2
+  q = fma2(q, f, pair(1.0f, 1.0f));
+  const float2 ti = split(t), r = split(q);
+  const float a = __int_as_float(__float_as_int(r.x) + (__float_as_int(ti.x) << 23));
+  const float b = __int_as_float(__float_as_int(r.y) + (__float_as_int(ti.y) << 23));
+  return pair(u.x < -126.0f ? 0.0f : u.x != u.x ? u.x : a, u.y < -126.0f ? 0.0f : u.y != u.y ? u.y : b);
+}
+
+// Exponentials of one row. `c` is log2(e) / T for the distillation term, `c1` log2(e) for the label term.
 template <int kMode>
 struct Exps {
   float cT, c1;
   int squarings;
-  __device__ __forceinline__ float numerator1(float v, float e, float n1) const {  // of the label term
+  // reference of the label term's exponentials that goes with reference `ref` (a logit) of the others
+  __device__ __forceinline__ float n1_of(float ref) const { return __fmul_rn(ref, c1); }
+  __device__ __forceinline__ uint64_t numerators1(uint64_t v, uint64_t e, float n1) const {
     if constexpr (kMode == kSquares) {
-      const float e2 = e * e;
-      return squarings == 2 ? e2 * e2 : e2;
+      const uint64_t e2 = mul2(e, e);
+      return squarings == 2 ? mul2(e2, e2) : e2;
     }
-    if constexpr (kMode == kTwoExps) return ex2(fmaf(v, c1, -n1));
+    if constexpr (kMode == kTwoExps) return ex2_pair_fma(fma2(v, pair(c1, c1), pair(-n1, -n1)));
     return e;
   }
-  __device__ __forceinline__ void add(float v, float n, float n1, float& s, float& s1) const {
-    const float e = ex2(fmaf(v, cT, -n));
-    s += e;
-    if constexpr (kMode != kOneExp) s1 += numerator1(v, e, n1);
+  __device__ __forceinline__ void add(uint64_t v, float n, float n1, uint64_t& s, uint64_t& s1) const {
+    const uint64_t e = ex2_pair(fma2(v, pair(cT, cT), pair(-n, -n)));
+    s = add2(s, e);
+    if constexpr (kMode != kOneExp) s1 = add2(s1, numerators1(v, e, n1));
   }
-  __device__ __forceinline__ float grad(float v, const RowStats& r) const {
-    const float e = ex2(fmaf(v, cT, -r.n));
-    if constexpr (kMode == kOneExp) return e * r.kT;  // kT holds both factors
-    return e * r.kT + numerator1(v, e, r.n1) * r.k1;
+  __device__ __forceinline__ uint64_t grad(uint64_t v, const RowStats& r) const {
+    const uint64_t e = ex2_pair(fma2(v, pair(cT, cT), pair(-r.n, -r.n)));
+    if constexpr (kMode == kOneExp) return mul2(e, pair(r.kT, r.kT));  // kT holds both factors
+    if constexpr (kMode == kSquares) {
+      if (squarings == 1) return mul2(e, fma2(e, pair(r.k1, r.k1), pair(r.kT, r.kT)));
+    }
+    return fma2(numerators1(v, e, r.n1), pair(r.k1, r.k1), mul2(e, pair(r.kT, r.kT)));
   }
+  __device__ __forceinline__ float grad1(float v, const RowStats& r) const { return split(grad(pair(v, v), r)).x; }
 };
+
+// A packet's values as pairs, and back.
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const Pack16<T>& p, uint64_t (&v)[Pack16<T>::kN / 2]) {
+  float f[Pack16<T>::kN];
+  unpack16(p, f);
+#pragma unroll
+  for (int i = 0; i < Pack16<T>::kN / 2; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
+}
+template <typename T>
+__device__ __forceinline__ Pack16<T> pack_pairs(const uint64_t (&v)[Pack16<T>::kN / 2]) {
+  float f[Pack16<T>::kN];
+#pragma unroll
+  for (int i = 0; i < Pack16<T>::kN / 2; ++i) {
+    const float2 t = split(v[i]);
+    f[2 * i] = t.x, f[2 * i + 1] = t.y;
+  }
+  Pack16<T> o;
+  pack16(o, f);
+  return o;
+}
+template <typename T>
+__device__ __forceinline__ Pack16<T> zero_packet() {
+  Pack16<T> o;
+  *reinterpret_cast<int4*>(&o) = make_int4(0, 0, 0, 0);
+  return o;
+}
 
 // An entry of a row's list (k < K) or its label (k = K): column or -1, teacher logit, own logit.
 template <typename T>
@@ -249,12 +338,16 @@ __device__ __forceinline__ float cross_term(const RowStats& r, float cT, float t
   const float a = fmaf(t, cT, -r.nt), pk = ex2(a) / r.St;
   return pk != 0.0f ? pk * (kLn2 * (a - fmaf(zv, cT, -r.n))) : 0.0f;
 }
-__device__ __forceinline__ float row_loss(const DistillParams& p, const RowStats& r, float cross, float z_label, float c1) {
-  constexpr float kLn2 = 0.6931471805599453f;
+// The loss is what the sums contribute plus what the list's and the label's own logits do.
+__device__ __forceinline__ float loss_of_sums(const DistillParams& p, const RowStats& r) {
   float loss = 0.0f;
-  if (r.some) loss = (1.0f - p.alpha) * p.temperature * p.temperature * (cross - logf(r.St) + logf(r.S));
-  if (r.known) loss += p.alpha * (logf(r.S1) - kLn2 * fmaf(z_label, c1, -r.n1));
+  if (r.some) loss = (1.0f - p.alpha) * p.temperature * p.temperature * (logf(r.S) - logf(r.St));
+  if (r.known) loss += p.alpha * logf(r.S1);
   return loss;
+}
+__device__ __forceinline__ float label_term(const DistillParams& p, const RowStats& r, float z_label, float c1) {
+  constexpr float kLn2 = 0.6931471805599453f;
+  return -p.alpha * (kLn2 * fmaf(z_label, c1, -r.n1));
 }
 __device__ __forceinline__ float max_of(const Pack16<float>& v) { return fmaxf(fmaxf(v.v[0], v.v[1]), fmaxf(v.v[2], v.v[3])); }
 __device__ __forceinline__ float max_of(const Pack16<__nv_bfloat16>& v) {
@@ -336,56 +429,54 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) distill_warp_kernel(const 
   m = warp_max(m);
   RowStats r;
   const float ref = m == -INFINITY ? 0.0f : m;
-  r.n = ref * x.cT;
-  r.n1 = kMode == kSquares ? r.n * p.temperature : ref * x.c1;
-  float s = 0.0f, s1 = 0.0f;
+  r.n = __fmul_rn(ref, x.cT);
+  r.n1 = x.n1_of(ref);
+  uint64_t s2 = pair(0.0f, 0.0f), s12 = s2;
+  if (edges > 0) x.add(pair(fe, -INFINITY), r.n, r.n1, s2, s12);  // lanes without an edge element add zeros
 #pragma unroll
   for (int q = 0; q < kPk; ++q)
     if (lane + 32 * q < pn) {
-      float f[kN];
-      unpack16(raw[q], f);
+      uint64_t v[kN / 2];
+      unpack_pairs<T>(raw[q], v);
 #pragma unroll
-      for (int e = 0; e < kN; ++e) x.add(f[e], r.n, r.n1, s, s1);
+      for (int e = 0; e < kN / 2; ++e) x.add(v[e], r.n, r.n1, s2, s12);
     }
-  if (edge_col >= 0) x.add(fe, r.n, r.n1, s, s1);
-  r.S = warp_sum(s);
-  r.S1 = kMode == kOneExp ? r.S : warp_sum(s1);
+  {
+    const float2 a = split(s2), b = split(s12);
+    r.S = warp_sum(a.x + a.y);
+    r.S1 = kMode == kOneExp ? r.S : warp_sum(b.x + b.y);
+  }
   r.nt = warp_max(nt);
   r.St = warp_sum(nt == -INFINITY ? st : st * rescale(nt, r.nt));
   __syncwarp();
   finish_stats(p, kMode, hard && col_s[p.K] >= 0, r);
-  if (r.some || r.known) {
-    float cross = 0.0f;
-    if (r.some) {
-      for (int k = lane; k < p.K; k += 32)
-        if (col_s[k] >= 0) cross += cross_term(r, x.cT, t_s[k], z_s[k]);
-      cross = warp_sum(cross);
-    }
-    if (lane == 0) p.loss[row] = row_loss(p, r, cross, z_s[p.K], x.c1);
-  } else if (lane == 0) {
-    p.loss[row] = 0.0f;
+  float own = 0.0f;
+  if (r.some) {
+    for (int k = lane; k < p.K; k += 32)
+      if (col_s[k] >= 0) own += cross_term(r, x.cT, t_s[k], z_s[k]);
+    own = (1.0f - p.alpha) * p.temperature * p.temperature * warp_sum(own);
   }
+  if (lane == 0) p.loss[row] = loss_of_sums(p, r) + own + (r.known ? label_term(p, r, z_s[p.K], x.c1) : 0.0f);
   if (!p.dz) return;
   T* out = static_cast<T*>(p.dz) + row * p.lddz;
   PK* out_packets = reinterpret_cast<PK*>(out + head);
-  const bool dead = !r.some && !r.known;
+  if (!r.some && !r.known) {  // neither term: zeros, whatever the logits hold
+#pragma unroll
+    for (int q = 0; q < kPk; ++q)
+      if (lane + 32 * q < pn) st_stream(out_packets + lane + 32 * q, zero_packet<T>());
+    if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(0.0f);
+    return;
+  }
 #pragma unroll
   for (int q = 0; q < kPk; ++q)
     if (lane + 32 * q < pn) {
-      float f[kN];
-      unpack16(raw[q], f);
+      uint64_t v[kN / 2];
+      unpack_pairs<T>(raw[q], v);
 #pragma unroll
-      for (int e = 0; e < kN; ++e) f[e] = x.grad(f[e], r);
-      if (dead) {
-#pragma unroll
-        for (int e = 0; e < kN; ++e) f[e] = 0.0f;
-      }
-      PK o;
-      pack16(o, f);
-      st_stream(out_packets + lane + 32 * q, o);
+      for (int e = 0; e < kN / 2; ++e) v[e] = x.grad(v[e], r);
+      st_stream(out_packets + lane + 32 * q, pack_pairs<T>(v));
     }
-  if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(dead ? 0.0f : x.grad(fe, r));
-  if (dead) return;
+  if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(x.grad1(fe, r));
   const bool dup = __any_sync(0xffffffffu, twice);
   __syncwarp();  // the corrections come behind the row: other lanes, the same addresses
   for (int k = lane; k < entries; k += 32) {
@@ -402,7 +493,7 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) distill_warp_kernel(const 
     } else {
       w = entry_weight(p, r, x.cT, k, t_s[k]);
     }
-    if (first) out[col] = Cvt<T>::from_f(x.grad(z_s[k], r) - w);
+    if (first) out[col] = Cvt<T>::from_f(x.grad1(z_s[k], r) - w);
   }
 }
 
@@ -447,7 +538,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
   uint32_t* bits_s = reinterpret_cast<uint32_t*>(dsmem + static_cast<size_t>(g.slice) * 16 + 16);
   int* col_all = reinterpret_cast<int*>(bits_s + 2 * words);
   __shared__ float red[2][5][kRowThreads / 32];
-  __shared__ float peer[2][kMaxRanks][3];
+  __shared__ float peer[2][kMaxRanks][4];  // per CTA of the cluster: maximum, two sums, and its part of the loss
   __shared__ int twice[2];    // some column occurs more than once
   __shared__ int wait_failed;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x, nwarps = nthreads >> 5;
@@ -471,6 +562,18 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
       sm100::bulk_copy_g2s(buf, z + head + static_cast<int64_t>(p0) * kN, static_cast<uint32_t>(n) * 16, bar);
     }
   };
+  // what a thread reads of a row from global memory itself: entry `tid` of its list, and an element outside the packets
+  // (rank 0 has those). Asked for one row ahead.
+  auto list_id = [&](int64_t row, int k) { return k < p.K ? __ldg(p.ids + row * p.K + k) : hard ? __ldg(p.labels + row) : -1; };
+  auto list_t = [&](int64_t row, int k) { return k < p.K ? teacher_at(p, row * p.K + k) : 0.0f; };
+  auto edge_of = [&](int64_t row) {
+    const int head = head_elements(static_cast<const T*>(p.z) + row * p.ldz, p.C), tail0 = head + (C - head) / kN * kN;
+    const int edges = rank == 0 ? head + C - tail0 : 0;
+    return tid < edges ? (tid < head ? tid : tail0 + tid - head) : -1;
+  };
+  auto edge_value = [&](int64_t row, int col) {
+    return col >= 0 ? Cvt<T>::to_f(static_cast<const T*>(p.z)[row * p.ldz + col]) : -INFINITY;
+  };
 
   if (tid == 0) {
     sm100::mbar_init(bar, 1);
@@ -480,70 +583,100 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
   }
   for (int i = tid; i < 2 * words; i += nthreads) bits_s[i] = 0u;
   __syncthreads();
-  if (tid == 0 && first_row < p.B) fetch(first_row);
+  int my_id = -1;
+  float my_t = 0.0f, my_edge = -INFINITY;
+  if (first_row < p.B) {
+    if (tid == 0) fetch(first_row);
+    if (tid < entries) my_id = list_id(first_row, tid), my_t = list_t(first_row, tid);
+    my_edge = edge_value(first_row, edge_of(first_row));
+  }
   bool piped = true;  // false once a copy did not arrive: the remaining rows run on what the buffer holds
   uint32_t phase = 0;
   int par = 0;
+  int64_t owed = -1;  // cluster: the row whose loss waits for the other CTAs' parts
+  float owed_base = 0.0f;
   for (int64_t row = first_row; row < p.B; row += row_step, par ^= 1) {
     const T* z = static_cast<const T*>(p.z) + row * p.ldz;
     const int head = head_elements(z, p.C), pn = packets_of(head);
     const int tail0 = head + (C - head) / kN * kN;
-    const int edges = rank == 0 ? head + C - tail0 : 0;  // rank 0 has the elements outside the packets
-    const int edge_col = tid < edges ? (tid < head ? tid : tail0 + tid - head) : -1;
-    const float fe = edge_col >= 0 ? Cvt<T>::to_f(z[edge_col]) : -INFINITY;
+    const int edge_col = edge_of(row);
+    const float fe = my_edge;
     uint32_t* bits = bits_s + par * words;
     int* col_s = col_all + par * 3 * entries;
     float* t_s = reinterpret_cast<float*>(col_s + entries);
     float* z_s = t_s + entries;
-    // the place of a column in this CTA's marks, -1 for another CTA's column
+    // the place of a column among this CTA's elements, -1 for another CTA's column
     auto place = [&](int col) {
+      if (col < 0) return -1;
       if (col < head) return rank == 0 ? g.slice * kN + col : -1;
       if (col >= tail0) return rank == 0 ? g.slice * kN + kN + col - tail0 : -1;
       const int at = col - head - p0 * kN;
       return at >= 0 && at < pn * kN ? at : -1;
     };
-    // the row's list, while the row itself is on its way
+    // the row's list: every CTA of a cluster has all of it, marks its own columns and sums the teacher's weights
     float nt = -INFINITY, st = 0.0f;
     for (int k = tid; k < entries; k += nthreads) {
-      int col;
-      float t, zv;
-      load_entry<T>(p, hard, row, k, &col, &t, &zv);
+      const int id = k == tid ? my_id : list_id(row, k);
+      const float t = k == tid ? my_t : list_t(row, k);
+      const int col = id >= 0 && id < C ? id : -1;
       col_s[k] = col;
       t_s[k] = t;
-      z_s[k] = zv;
-      if (col >= 0) {
-        if (k < p.K) teacher_add(t, x.cT, nt, st);
-        const int at = p.dz ? place(col) : -1;
-        if (at >= 0 && (atomicOr(bits + (at >> 5), 1u << (at & 31)) & (1u << (at & 31)))) twice[par] = 1;
-      }
+      if (col >= 0 && k < p.K) teacher_add(t, x.cT, nt, st);
+      const int at = place(col);
+      if (p.dz && at >= 0 && (atomicOr(bits + (at >> 5), 1u << (at & 31)) & (1u << (at & 31)))) twice[par] = 1;
     }
     if (pn > 0 && piped) {
       if (!sm100::mbar_wait_bounded(bar, phase, rowk::kRowWaitBudgetNs)) wait_failed = 1;
       phase ^= 1u;
     }
-    float m = fe;
-#pragma unroll 4
-    for (int pi = tid; pi < pn; pi += nthreads) m = fmaxf(m, max_of(row_s[pi]));
-    m = warp_max(m);
+    for (int k = tid; k < entries; k += nthreads) {
+      const int col = col_s[k], at = place(col);
+      if (at >= 0) z_s[k] = at < g.slice * kN ? Cvt<T>::to_f(reinterpret_cast<const T*>(dsmem)[at]) : Cvt<T>::to_f(z[col]);
+    }
+    // Maximum and sums in one pass, kGroup packets at a time: a larger maximum rescales the sums so far, which after the
+    // first groups hardly happens.
+    constexpr int kGroup = 2;
+    float m = -INFINITY, n = 0.0f, n1 = 0.0f;
+    uint64_t s2 = pair(0.0f, 0.0f), s12 = s2;
+    auto raise = [&](float to) {
+      if (to > m) {
+        const float nn = __fmul_rn(to, x.cT), nn1 = x.n1_of(to);
+        const float k = m == -INFINITY ? 0.0f : rescale(n, nn), k1 = m == -INFINITY ? 0.0f : rescale(n1, nn1);
+        s2 = mul2(s2, pair(k, k));
+        if constexpr (kMode != kOneExp) s12 = mul2(s12, pair(k1, k1));
+        m = to, n = nn, n1 = nn1;
+      }
+    };
+    if (edge_col >= 0) {
+      raise(fe);
+      x.add(pair(fe, -INFINITY), n, n1, s2, s12);
+    }
+    for (int pi = tid; pi < pn; pi += kGroup * nthreads) {
+      PK v[kGroup];
+      v[0] = row_s[pi];
+      const bool two = pi + nthreads < pn;
+      if (two) v[1] = row_s[pi + nthreads];
+      const float a = max_of(v[0]);
+      raise(two ? fmaxf(a, max_of(v[1])) : a);
+#pragma unroll
+      for (int q = 0; q < kGroup; ++q)
+        if (q == 0 || two) {
+          uint64_t f[kN / 2];
+          unpack_pairs<T>(v[q], f);
+#pragma unroll
+          for (int e = 0; e < kN / 2; ++e) x.add(f[e], n, n1, s2, s12);
+        }
+    }
     RowStats r;
     {
-      const float ref = m == -INFINITY ? 0.0f : m;
-      const float n = ref * x.cT, n1 = kMode == kSquares ? n * p.temperature : ref * x.c1;
-      float s = 0.0f, s1 = 0.0f;
-#pragma unroll 2
-      for (int pi = tid; pi < pn; pi += nthreads) {
-        float f[kN];
-        unpack16(row_s[pi], f);
-#pragma unroll
-        for (int e = 0; e < kN; ++e) x.add(f[e], n, n1, s, s1);
-      }
-      if (edge_col >= 0) x.add(fe, n, n1, s, s1);
-      s = warp_sum(s);
-      if constexpr (kMode != kOneExp) s1 = warp_sum(s1);
-      const float ntw = warp_max(nt);
+      const float mw = warp_max(m), ntw = warp_max(nt);
+      const float nw = mw == -INFINITY ? 0.0f : __fmul_rn(mw, x.cT), nw1 = mw == -INFINITY ? 0.0f : x.n1_of(mw);
+      const float2 a = split(s2), b = split(s12);
+      const float s = warp_sum((a.x + a.y) * (m == -INFINITY ? 1.0f : rescale(n, nw)));  // nothing added yet: 0, or NaN
+      const float s1 = kMode == kOneExp ? 0.0f : warp_sum((b.x + b.y) * (m == -INFINITY ? 1.0f : rescale(n1, nw1)));
       st = warp_sum(nt == -INFINITY ? st : st * rescale(nt, ntw));
       if (lane == 0) {
-        red[par][0][warp] = m;
+        red[par][0][warp] = mw;
         red[par][1][warp] = s;
         red[par][2][warp] = s1;
         red[par][3][warp] = ntw;
@@ -558,7 +691,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
       m = warp_max(a);
       r.nt = warp_max(at);
       r.S = warp_sum(in ? red[par][1][lane] * (a == m ? 1.0f : ex2(__fmul_rn(a, x.cT) - __fmul_rn(m, x.cT))) : 0.0f);
-      r.S1 = kMode == kOneExp ? r.S : warp_sum(in ? red[par][2][lane] * (a == m ? 1.0f : ex2(__fmul_rn(a, x.c1) - __fmul_rn(m, x.c1))) : 0.0f);
+      r.S1 = kMode == kOneExp ? r.S : warp_sum(in ? red[par][2][lane] * (a == m ? 1.0f : ex2(x.n1_of(a) - x.n1_of(m))) : 0.0f);
       r.St = warp_sum(in ? red[par][4][lane] * rescale(at, r.nt) : 0.0f);
     }
     if (g.ranks > 1) {
@@ -575,58 +708,69 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
       for (int k = 0; k < g.ranks; ++k) {
         const float pm = peer[par][k][0];
         r.S += peer[par][k][1] * (pm == a ? 1.0f : ex2(__fmul_rn(pm, x.cT) - __fmul_rn(a, x.cT)));
-        r.S1 += peer[par][k][2] * (pm == a ? 1.0f : ex2(__fmul_rn(pm, x.c1) - __fmul_rn(a, x.c1)));
+        r.S1 += peer[par][k][2] * (pm == a ? 1.0f : ex2(x.n1_of(pm) - x.n1_of(a)));
       }
       m = a;
       if constexpr (kMode == kOneExp) r.S1 = r.S;
+      if (rank == 0 && tid == 0 && owed >= 0) {  // the parts of the row before have arrived behind this barrier
+        for (int k = 0; k < g.ranks; ++k) owed_base += peer[par ^ 1][k][3];
+        p.loss[owed] = owed_base;
+      }
     }
     {
       const float ref = m == -INFINITY ? 0.0f : m;
-      r.n = ref * x.cT;
-      r.n1 = kMode == kSquares ? r.n * p.temperature : ref * x.c1;
+      r.n = __fmul_rn(ref, x.cT);
+      r.n1 = x.n1_of(ref);
     }
     finish_stats(p, kMode, hard && col_s[p.K] >= 0, r);
     const bool dead = !r.some && !r.known;
     T* out = static_cast<T*>(p.dz) + row * p.lddz;
     if (p.dz) {
       PK* packets = reinterpret_cast<PK*>(out + head) + p0;
+      if (dead) {  // neither term: zeros, whatever the logits hold
+        for (int pi = tid; pi < pn; pi += nthreads) st_stream(packets + pi, zero_packet<T>());
+      } else {
 #pragma unroll 2
-      for (int pi = tid; pi < pn; pi += nthreads) {
-        float f[kN];
-        unpack16(row_s[pi], f);
+        for (int pi = tid; pi < pn; pi += nthreads) {
+          uint64_t f[kN / 2];
+          unpack_pairs<T>(row_s[pi], f);
 #pragma unroll
-        for (int e = 0; e < kN; ++e) f[e] = x.grad(f[e], r);
-        if (dead) {
-#pragma unroll
-          for (int e = 0; e < kN; ++e) f[e] = 0.0f;
+          for (int e = 0; e < kN / 2; ++e) f[e] = x.grad(f[e], r);
+          st_stream(packets + pi, pack_pairs<T>(f));
         }
-        PK o;
-        pack16(o, f);
-        st_stream(packets + pi, o);
       }
-      if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(dead ? 0.0f : x.grad(fe, r));
+      if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(dead ? 0.0f : x.grad1(fe, r));
       if (tid == 0) twice[par ^ 1] = 0;  // last read one row ago, next set behind this barrier
     }
     __syncthreads();  // the buffer is free; the corrections below come behind the row's stores
     if (wait_failed) piped = false;
-    if (tid == 0 && row + row_step < p.B && piped) {
-      sm100::fence_generic_to_async_smem();
-      fetch(row + row_step);
+    const int64_t next = row + row_step;
+    if (next < p.B) {
+      if (tid == 0 && piped) {
+        sm100::fence_generic_to_async_smem();
+        fetch(next);
+      }
+      if (tid < entries) my_id = list_id(next, tid), my_t = list_t(next, tid);
+      my_edge = edge_value(next, edge_of(next));
     }
-    if (rank == 0 && warp == nwarps - 1) {
-      float cross = 0.0f;
+    if (warp == nwarps - 1) {  // this CTA's part of the loss: its own columns' logits
+      float own = 0.0f;
       if (r.some) {
         for (int k = lane; k < p.K; k += 32)
-          if (col_s[k] >= 0) cross += cross_term(r, x.cT, t_s[k], z_s[k]);
-        cross = warp_sum(cross);
+          if (place(col_s[k]) >= 0) own += cross_term(r, x.cT, t_s[k], z_s[k]);
+        own = (1.0f - p.alpha) * p.temperature * p.temperature * warp_sum(own);
       }
-      if (lane == 0) p.loss[row] = row_loss(p, r, cross, z_s[p.K], x.c1);
+      if (lane == 0) {
+        if (r.known && place(col_s[p.K]) >= 0) own += label_term(p, r, z_s[p.K], x.c1);
+        if (g.ranks > 1) st_peer_shared(&peer[par][rank][3], 0, own);
+        else p.loss[row] = loss_of_sums(p, r) + own;
+      }
     }
+    if (rank == 0 && tid == 0 && g.ranks > 1) owed = row, owed_base = loss_of_sums(p, r);
     if (p.dz) {
       const bool dup = twice[par] != 0;
       for (int k = tid; k < entries; k += nthreads) {
-        const int col = col_s[k];
-        const int at = col >= 0 ? place(col) : -1;
+        const int col = col_s[k], at = place(col);
         if (at < 0) continue;
         bits[at >> 5] = 0u;  // this row's marks go
         float w = 0.0f;
@@ -640,11 +784,17 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
         } else {
           w = entry_weight(p, r, x.cT, k, t_s[k]);
         }
-        if (first) out[col] = Cvt<T>::from_f(x.grad(z_s[k], r) - w);
+        if (first) out[col] = Cvt<T>::from_f(x.grad1(z_s[k], r) - w);
       }
     }
   }
-  if (g.ranks > 1) cluster_barrier();  // nobody leaves while a peer may still write its shared memory
+  if (g.ranks > 1) {
+    cluster_barrier();  // nobody leaves while a peer may still write its shared memory
+    if (rank == 0 && tid == 0 && owed >= 0) {
+      for (int k = 0; k < g.ranks; ++k) owed_base += peer[par ^ 1][k][3];
+      p.loss[owed] = owed_base;
+    }
+  }
   if (wait_failed) {
     if (tid == 0) atomicExch(&g_distill_status, 1);
     for (int i = 0; i < 64; ++i) __nanosleep(16384);  // error path only: let a late copy land
@@ -710,16 +860,34 @@ Status launch_block_rows(const DistillParams& p, const RowPlan& g, cudaStream_t 
   // registers allow kRowCtas blocks of kRowThreads threads
   int resident = rowk::row_pipe_blocks_per_sm(g.threads, g.smem + 1024);
   if (resident > kRowCtas * kRowThreads / g.threads) resident = kRowCtas * kRowThreads / g.threads;
-  int over = 1;
-  if (const char* e = std::getenv("AICF_DISTILL_OVER")) over = std::atoi(e);
-  const int64_t slots = static_cast<int64_t>(sm_count()) * resident * over / g.ranks;
-  const int64_t rows = p.B < slots ? p.B : (slots > 0 ? slots : 1);
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * g.ranks));
   cfg.blockDim = dim3(static_cast<unsigned>(g.threads));
   cfg.dynamicSmemBytes = g.smem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = g.ranks > 1 ? 1 : 0;
+  int64_t slots = static_cast<int64_t>(sm_count()) * resident / g.ranks;
+  if (g.ranks > 1) {
+    // Clusters do not fill every SM (a cluster stays inside one group of SMs): a grid larger than what fits at once would
+    // run its last clusters as a second wave. Asked of the runtime once per shape.
+    static std::mutex mu;
+    static std::map<std::array<int64_t, 4>, int> known;
+    const std::array<int64_t, 4> key{device_slot(), g.ranks, g.threads, static_cast<int64_t>(g.smem)};
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = known.find(key);
+    if (it == known.end()) {
+      cfg.gridDim = dim3(static_cast<unsigned>(sm_count() * resident / g.ranks * g.ranks));
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = static_cast<int>(slots > 0 ? slots : 1);
+      }
+      if (known.size() > 256) known.clear();
+      it = known.emplace(key, n).first;
+    }
+    if (it->second < slots) slots = it->second;
+  }
+  const int64_t rows = p.B < slots ? p.B : (slots > 0 ? slots : 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * g.ranks));
   if (cudaLaunchKernelEx(&cfg, kernel, p, g) != cudaSuccess) {
     cudaGetLastError();
     return Status::Internal;
