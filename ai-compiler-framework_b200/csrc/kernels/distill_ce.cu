@@ -15,7 +15,6 @@
 // gradient both times). The same column may stand in a row's list more than once. loss_row carries no `scale`.
 // A row without either term gets zeros whatever its logits hold. dz may be z itself; otherwise outputs do not overlap inputs.
 #include <array>
-#include <cstdlib>
 #include <map>
 #include <mutex>
 
@@ -42,6 +41,8 @@ struct DistillParams {
   int64_t B, C;
   int K;
   float scale, temperature, alpha;
+  // from these: log2(e) / T; the weights of both terms in the gradient, scale (1 - alpha) T and scale alpha; (1 - alpha) T^2
+  float cT, grad_soft, grad_hard, loss_soft;
 };
 
 __device__ __forceinline__ float teacher_at(const DistillParams& p, int64_t i) {
@@ -155,7 +156,8 @@ __global__ void __launch_bounds__(256) distill_multipass_kernel(const DistillPar
 // costs three instructions. The three kinds of row differ in who holds it:
 //
 //   distill_warp_kernel    up to 2048 columns: one warp per row, the row in its registers, many short blocks
-//   distill_block_kernel   longer rows: one CTA, or one per slice of the row in a cluster, the slice in shared memory
+//   distill_block_kernel   longer rows: one CTA, or one per slice of the row in a cluster, the slice in shared memory; two or
+//                          three CTAs per SM in different phases keep loads, exponentials and stores going side by side
 //   distill_multipass_kernel  z and dz misaligned against each other, or a row past eight slices
 //
 // A row may start anywhere: the whole 16-byte packets inside it are handled as packets, the up to 2 * (kN - 1) elements
@@ -167,9 +169,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// 2^(from - to), 1 for equal references (two of -inf, two of +inf)
-__device__ __forceinline__ float rescale(float from, float to) { return from == to ? 1.0f : ex2(from - to); }
-
 // How the exponentials of the two softmaxes come about.
 enum ExpMode : int {
   kOneExp = 0,    // no label term, or T = 1: one exponential serves both
@@ -216,28 +215,6 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t v) {
   const float2 u = split(v);
   return pair(ex2(u.x), ex2(u.y));
 }
-// 2^u for u <= 0 on the FMA pipe: u = i + f with i the nearest integer, 2^f by its Taylor polynomial of degree 6 (|f| <= 1/2:
-// off by at most (ln2 / 2)^7 / 7! = 1.2e-7), i added to the exponent. Below 2^-126 the result is 0; a NaN stays one. Rows with
-// two exponentials per logit take one of them here, because the special-function unit serves four lanes per clock and
-// scheduler only.
-__device__ __forceinline__ uint64_t ex2_pair_fma(uint64_t v) {
-  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the integer lands in the low mantissa bits
-  const float2 u = split(v);
-  const uint64_t t = add2(v, pair(kMagic, kMagic));
-  const uint64_t f = add2(v, mul2(add2(t, pair(-kMagic, -kMagic)), pair(-1.0f, -1.0f)));
-  uint64_t q = pair(1.54035303933816e-4f, 1.54035303933816e-4f);                        // ln2^6 / 6!
-  q = fma2(q, f, pair(1.33335581464284e-3f, 1.33335581464284e-3f));                     // ln2^5 / 5!
-  q = fma2(q, f, pair(9.61812910762848e-3f, 9.61812910762848e-3f));                     // ln2^4 / 4!
-  q = fma2(q, f, pair(5.55041086648216e-2f, 5.55041086648216e-2f));                     // ln2^3 / 3!
-  q = fma2(q, f, pair(2.40226506959101e-1f, 2.40226506959101e-1f));                     // ln2^2 / 2
-  q = fma2(q, f, pair(6.93147180559945e-1f, 6.93147180559945e-1f));                     // ln2
-  q = fma2(q, f, pair(1.0f, 1.0f));
-  const float2 ti = split(t), r = split(q);
-  const float a = __int_as_float(__float_as_int(r.x) + (__float_as_int(ti.x) << 23));
-  const float b = __int_as_float(__float_as_int(r.y) + (__float_as_int(ti.y) << 23));
-  return pair(u.x < -126.0f ? 0.0f : u.x != u.x ? u.x : a, u.y < -126.0f ? 0.0f : u.y != u.y ? u.y : b);
-}
-
 // Exponentials of one row. `c` is log2(e) / T for the distillation term, `c1` log2(e) for the label term.
 template <int kMode>
 struct Exps {
@@ -250,7 +227,7 @@ struct Exps {
       const uint64_t e2 = mul2(e, e);
       return squarings == 2 ? mul2(e2, e2) : e2;
     }
-    if constexpr (kMode == kTwoExps) return ex2_pair_fma(fma2(v, pair(c1, c1), pair(-n1, -n1)));
+    if constexpr (kMode == kTwoExps) return ex2_pair(fma2(v, pair(c1, c1), pair(-n1, -n1)));
     return e;
   }
   __device__ __forceinline__ void add(uint64_t v, float n, float n1, uint64_t& s, uint64_t& s1) const {
@@ -296,57 +273,37 @@ __device__ __forceinline__ Pack16<T> zero_packet() {
   return o;
 }
 
-// An entry of a row's list (k < K) or its label (k = K): column or -1, teacher logit, own logit.
-template <typename T>
-__device__ __forceinline__ void load_entry(const DistillParams& p, bool hard, int64_t row, int k, int* col, float* t, float* zv) {
-  int id = -1;
-  *t = 0.0f;
-  *zv = 0.0f;
-  if (k < p.K) id = __ldg(p.ids + row * p.K + k);
-  else if (hard) id = __ldg(p.labels + row);
-  const bool ok = id >= 0 && id < p.C;
-  *col = ok ? id : -1;
-  if (ok) {
-    if (k < p.K) *t = teacher_at(p, row * p.K + k);
-    *zv = Cvt<T>::to_f(static_cast<const T*>(p.z)[row * p.ldz + id]);
-  }
-}
-// Running reference and sum of the teacher's weights.
-__device__ __forceinline__ void teacher_add(float t, float cT, float& nt, float& st) {
-  const float u = t * cT, to = fmaxf(nt, u);
-  const float ref = to == -INFINITY ? 0.0f : to;
-  st = st * (nt == -INFINITY ? 0.0f : rescale(nt, ref)) + ex2(u - ref);
-  nt = to;
-}
-__device__ __forceinline__ void finish_stats(const DistillParams& p, int mode, bool known, RowStats& r) {
+__device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }  // 2 ulp for b < 2^126; the sums are
+
+// From the sums to the factors of the numerators in the gradient.
+template <int kMode>
+__device__ __forceinline__ void finish_stats(const DistillParams& p, bool known, RowStats& r) {
   if (r.S == 0.0f) r.S = r.S1 = __int_as_float(0x7fc00000);  // a row of -inf has no softmax
-  if (r.nt == -INFINITY) r.nt = 0.0f;
   r.some = !(r.St == 0.0f);  // else no entries, or every entry has weight zero
   r.known = known;
-  r.kT = r.some ? p.scale * (1.0f - p.alpha) * p.temperature / r.S : 0.0f;
-  r.k1 = known ? p.scale * p.alpha / r.S1 : 0.0f;
-  if (mode == kOneExp) r.kT += r.k1;
+  r.kT = r.some ? quotient(p.grad_soft, r.S) : 0.0f;
+  r.k1 = known ? quotient(p.grad_hard, r.S1) : 0.0f;
+  if (kMode == kOneExp) r.kT += r.k1;
 }
-// The weight that entry j takes from the gradient at its column.
-__device__ __forceinline__ float entry_weight(const DistillParams& p, const RowStats& r, float cT, int j, float t) {
-  if (j == p.K) return p.scale * p.alpha;
-  return r.some ? p.scale * (1.0f - p.alpha) * p.temperature * (ex2(fmaf(t, cT, -r.nt)) / r.St) : 0.0f;
+// p_k
+__device__ __forceinline__ float target(const DistillParams& p, const RowStats& r, float t) {
+  return r.some ? quotient(ex2(fmaf(t, p.cT, -r.nt)), r.St) : 0.0f;
 }
-// p_k (log p_k - log q_k) without the sums' logarithms; natural logarithms
-__device__ __forceinline__ float cross_term(const RowStats& r, float cT, float t, float zv) {
-  constexpr float kLn2 = 0.6931471805599453f;
-  const float a = fmaf(t, cT, -r.nt), pk = ex2(a) / r.St;
-  return pk != 0.0f ? pk * (kLn2 * (a - fmaf(zv, cT, -r.n))) : 0.0f;
+// p_k (log2 p_k - log2 q_k) without the sums' logarithms
+__device__ __forceinline__ float cross_term(const DistillParams& p, const RowStats& r, float t, float zv) {
+  const float a = fmaf(t, p.cT, -r.nt), pk = target(p, r, t);
+  return pk != 0.0f ? pk * (a - fmaf(zv, p.cT, -r.n)) : 0.0f;
 }
-// The loss is what the sums contribute plus what the list's and the label's own logits do.
+// The loss is what the sums contribute plus what the list's (`cross`: the sum of cross_term) and the label's logits do.
 __device__ __forceinline__ float loss_of_sums(const DistillParams& p, const RowStats& r) {
   float loss = 0.0f;
-  if (r.some) loss = (1.0f - p.alpha) * p.temperature * p.temperature * (logf(r.S) - logf(r.St));
+  if (r.some) loss = p.loss_soft * logf(quotient(r.S, r.St));
   if (r.known) loss += p.alpha * logf(r.S1);
   return loss;
 }
-__device__ __forceinline__ float label_term(const DistillParams& p, const RowStats& r, float z_label, float c1) {
-  constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float loss_of_list(const DistillParams& p, float cross) { return p.loss_soft * (kLn2 * cross); }
+__device__ __forceinline__ float loss_of_label(const DistillParams& p, const RowStats& r, float z_label, float c1) {
   return -p.alpha * (kLn2 * fmaf(z_label, c1, -r.n1));
 }
 __device__ __forceinline__ float max_of(const Pack16<float>& v) { return fmaxf(fmaxf(v.v[0], v.v[1]), fmaxf(v.v[2], v.v[3])); }
@@ -377,49 +334,78 @@ struct RowPlan {
 
 constexpr int kRowsPerBlock = 8;
 
-// One warp per row.
-template <typename T, int kPk, int kMode>
-__global__ void __launch_bounds__(32 * kRowsPerBlock) distill_warp_kernel(const DistillParams p, const RowPlan g) {
+// One warp per row. kOneEach: the list with its label has at most 32 entries, one per lane and in registers; longer lists are
+// staged in shared memory next to a bit per column that finds repeated columns.
+template <typename T, int kPk, int kMode, bool kOneEach>
+__global__ void __launch_bounds__(32 * kRowsPerBlock, kPk * Pack16<T>::kN <= 32 ? 4 : 2) distill_warp_kernel(const DistillParams p, const RowPlan g) {
   using PK = Pack16<T>;
   constexpr int kN = PK::kN;
   extern __shared__ __align__(16) uint8_t dsmem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int entries = p.K + 1;
-  const int words = (static_cast<int>(p.C) + 31) / 32;
-  // per warp: marks of columns, then the row's list with its label: column, teacher logit, own logit
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + warp;
+  if (row >= p.B) return;  // whole warps: nothing below meets another warp
+  const bool hard = p.labels != nullptr && p.alpha > 0.0f;
+  const Exps<kMode> x{p.cT, kLog2e, g.squarings};
+  const T* z = static_cast<const T*>(p.z) + row * p.ldz;
+  const int C = static_cast<int>(p.C);
+  const int head = head_elements(z, p.C);
+  const int pn = (C - head) / kN, tail0 = head + pn * kN;
+  const int edges = head + C - tail0;
+  const PK* packets = reinterpret_cast<const PK*>(z + head) + lane;
+  PK raw[kPk];
+#pragma unroll
+  for (int q = 0; q < kPk; ++q)
+    if (lane + 32 * q < pn) raw[q] = ld_stream(packets + 32 * q);
+  // entry k of the row's list, or its label (k = K): column or -1, teacher logit, own logit
+  auto load_entry = [&](int k, int* col, float* t, float* zv) {
+    const int id = k < p.K ? __ldg(p.ids + row * p.K + k) : hard && k == p.K ? __ldg(p.labels + row) : -1;
+    *t = k < p.K ? teacher_at(p, row * p.K + k) : 0.0f;
+    *col = id >= 0 && id < C ? id : -1;
+    *zv = *col >= 0 ? Cvt<T>::to_f(z[id]) : 0.0f;
+  };
+  int my_col = -1;
+  float my_t = 0.0f, my_z = 0.0f;
+  if (lane < entries) load_entry(lane, &my_col, &my_t, &my_z);
+  int edge_col = -1;
+  float fe = -INFINITY;
+  if (edges > 0 && lane < edges) {
+    edge_col = lane < head ? lane : tail0 + lane - head;
+    fe = Cvt<T>::to_f(z[edge_col]);
+  }
+  const int words = (C + 31) / 32;
   uint32_t* bits_s = reinterpret_cast<uint32_t*>(dsmem) + warp * (words + 3 * entries);
   int* col_s = reinterpret_cast<int*>(bits_s + words);
   float* t_s = reinterpret_cast<float*>(col_s + entries);
   float* z_s = t_s + entries;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + warp;
-  if (row >= p.B) return;  // whole warps: nothing below meets another warp
-  const bool hard = p.labels != nullptr && p.alpha > 0.0f;
-  const Exps<kMode> x{kLog2e / p.temperature, kLog2e, g.squarings};
-  const T* z = static_cast<const T*>(p.z) + row * p.ldz;
-  const int head = head_elements(z, p.C);
-  const int pn = (static_cast<int>(p.C) - head) / kN, tail0 = head + pn * kN;
-  const int edges = head + static_cast<int>(p.C) - tail0;
-  const int edge_col = lane < edges ? (lane < head ? lane : tail0 + lane - head) : -1;
-  const PK* packets = reinterpret_cast<const PK*>(z + head);
-  PK raw[kPk];
-#pragma unroll
-  for (int q = 0; q < kPk; ++q)
-    if (lane + 32 * q < pn) raw[q] = ld_stream(packets + lane + 32 * q);
-  const float fe = edge_col >= 0 ? Cvt<T>::to_f(z[edge_col]) : -INFINITY;
-  for (int i = lane; i < words; i += 32) bits_s[i] = 0u;
-  __syncwarp();
+  RowStats r;
   bool twice = false;
-  float nt = -INFINITY, st = 0.0f;
-  for (int k = lane; k < entries; k += 32) {
-    int col;
-    float t, zv;
-    load_entry<T>(p, hard, row, k, &col, &t, &zv);
-    col_s[k] = col;
-    t_s[k] = t;
-    z_s[k] = zv;
-    if (col >= 0) {
-      if (k < p.K) teacher_add(t, x.cT, nt, st);
-      if (p.dz && (atomicOr(bits_s + (col >> 5), 1u << (col & 31)) & (1u << (col & 31)))) twice = true;
+  bool known;
+  {
+    float nt = my_col >= 0 && lane < p.K ? my_t * p.cT : -INFINITY;
+    if constexpr (kOneEach) {
+      r.nt = warp_max(nt);
+      if (r.nt == -INFINITY) r.nt = 0.0f;
+      r.St = warp_sum(my_col >= 0 && lane < p.K ? ex2(fmaf(my_t, p.cT, -r.nt)) : 0.0f);
+      known = __shfl_sync(0xffffffffu, my_col, p.K) >= 0;
+    } else {
+      for (int i = lane; i < words; i += 32) bits_s[i] = 0u;
+      __syncwarp();
+      for (int k = lane; k < entries; k += 32) {
+        if (k != lane) load_entry(k, &my_col, &my_t, &my_z);
+        col_s[k] = my_col, t_s[k] = my_t, z_s[k] = my_z;
+        if (my_col < 0) continue;
+        if (k < p.K) nt = fmaxf(nt, my_t * p.cT);
+        if (p.dz && (atomicOr(bits_s + (my_col >> 5), 1u << (my_col & 31)) & (1u << (my_col & 31)))) twice = true;
+      }
+      r.nt = warp_max(nt);
+      if (r.nt == -INFINITY) r.nt = 0.0f;
+      __syncwarp();
+      float st = 0.0f;
+      for (int k = lane; k < p.K; k += 32)
+        if (col_s[k] >= 0) st += ex2(fmaf(t_s[k], p.cT, -r.nt));
+      r.St = warp_sum(st);
+      known = col_s[p.K] >= 0;
     }
   }
   float m = fe;
@@ -427,9 +413,8 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) distill_warp_kernel(const 
   for (int q = 0; q < kPk; ++q)
     if (lane + 32 * q < pn) m = fmaxf(m, max_of(raw[q]));
   m = warp_max(m);
-  RowStats r;
   const float ref = m == -INFINITY ? 0.0f : m;
-  r.n = __fmul_rn(ref, x.cT);
+  r.n = __fmul_rn(ref, p.cT);
   r.n1 = x.n1_of(ref);
   uint64_t s2 = pair(0.0f, 0.0f), s12 = s2;
   if (edges > 0) x.add(pair(fe, -INFINITY), r.n, r.n1, s2, s12);  // lanes without an edge element add zeros
@@ -446,24 +431,29 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) distill_warp_kernel(const 
     r.S = warp_sum(a.x + a.y);
     r.S1 = kMode == kOneExp ? r.S : warp_sum(b.x + b.y);
   }
-  r.nt = warp_max(nt);
-  r.St = warp_sum(nt == -INFINITY ? st : st * rescale(nt, r.nt));
-  __syncwarp();
-  finish_stats(p, kMode, hard && col_s[p.K] >= 0, r);
+  finish_stats<kMode>(p, known, r);
   float own = 0.0f;
   if (r.some) {
-    for (int k = lane; k < p.K; k += 32)
-      if (col_s[k] >= 0) own += cross_term(r, x.cT, t_s[k], z_s[k]);
-    own = (1.0f - p.alpha) * p.temperature * p.temperature * warp_sum(own);
+    if constexpr (kOneEach) {
+      own = my_col >= 0 && lane < p.K ? cross_term(p, r, my_t, my_z) : 0.0f;
+    } else {
+      for (int k = lane; k < p.K; k += 32)
+        if (col_s[k] >= 0) own += cross_term(p, r, t_s[k], z_s[k]);
+    }
+    own = loss_of_list(p, warp_sum(own));
   }
-  if (lane == 0) p.loss[row] = loss_of_sums(p, r) + own + (r.known ? label_term(p, r, z_s[p.K], x.c1) : 0.0f);
+  if (known) {
+    if constexpr (kOneEach) own += loss_of_label(p, r, __shfl_sync(0xffffffffu, my_z, p.K), x.c1);
+    else own += loss_of_label(p, r, z_s[p.K], x.c1);
+  }
+  if (lane == 0) p.loss[row] = loss_of_sums(p, r) + own;
   if (!p.dz) return;
   T* out = static_cast<T*>(p.dz) + row * p.lddz;
-  PK* out_packets = reinterpret_cast<PK*>(out + head);
-  if (!r.some && !r.known) {  // neither term: zeros, whatever the logits hold
+  PK* out_packets = reinterpret_cast<PK*>(out + head) + lane;
+  if (!r.some && !known) {  // neither term: zeros, whatever the logits hold
 #pragma unroll
     for (int q = 0; q < kPk; ++q)
-      if (lane + 32 * q < pn) st_stream(out_packets + lane + 32 * q, zero_packet<T>());
+      if (lane + 32 * q < pn) st_stream(out_packets + 32 * q, zero_packet<T>());
     if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(0.0f);
     return;
   }
@@ -474,26 +464,46 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) distill_warp_kernel(const 
       unpack_pairs<T>(raw[q], v);
 #pragma unroll
       for (int e = 0; e < kN / 2; ++e) v[e] = x.grad(v[e], r);
-      st_stream(out_packets + lane + 32 * q, pack_pairs<T>(v));
+      st_stream(out_packets + 32 * q, pack_pairs<T>(v));
     }
   if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(x.grad1(fe, r));
-  const bool dup = __any_sync(0xffffffffu, twice);
-  __syncwarp();  // the corrections come behind the row: other lanes, the same addresses
-  for (int k = lane; k < entries; k += 32) {
-    const int col = col_s[k];
-    if (col < 0) continue;
-    float w = 0.0f;
-    bool first = true;
-    if (dup) {
-      for (int j = 0; j < entries; ++j)
-        if (col_s[j] == col) {
-          if (j < k) first = false;
-          w += entry_weight(p, r, x.cT, j, t_s[j]);
-        }
-    } else {
-      w = entry_weight(p, r, x.cT, k, t_s[k]);
+  // The corrections come behind the row: other lanes, the same addresses. Equal columns are corrected once, by their first
+  // entry, for the sum of their weights in the list's order.
+  if constexpr (kOneEach) {
+    float w = lane == p.K ? p.grad_hard : p.grad_soft * target(p, r, my_t);
+    bool first = my_col >= 0;
+    const uint32_t same = __match_any_sync(0xffffffffu, first ? my_col : -1 - lane);
+    if (__any_sync(0xffffffffu, (same & (same - 1)) != 0u)) {
+      const float mine = w;
+      w = 0.0f;
+      for (int j = 0; j < entries; ++j) {
+        const float other = __shfl_sync(0xffffffffu, mine, j);
+        if ((same >> j) & 1u) w += other;
+      }
+      first = first && lane == __ffs(static_cast<int>(same)) - 1;
     }
-    if (first) out[col] = Cvt<T>::from_f(x.grad1(z_s[k], r) - w);
+    __syncwarp();
+    if (first) out[my_col] = Cvt<T>::from_f(x.grad1(my_z, r) - w);
+  } else {
+    const bool dup = __any_sync(0xffffffffu, twice);
+    __syncwarp();
+    for (int k = lane; k < entries; k += 32) {
+      const int col = col_s[k];
+      if (col < 0) continue;
+      float w = 0.0f;
+      bool first = true;
+      auto weight = [&](int j) { return j == p.K ? p.grad_hard : p.grad_soft * target(p, r, t_s[j]); };
+      if (dup) {
+        for (int j = 0; j < entries; ++j)
+          if (col_s[j] == col) {
+            if (j < k) first = false;
+            w += weight(j);
+          }
+      } else {
+        w = weight(k);
+      }
+      if (first) out[col] = Cvt<T>::from_f(x.grad1(z_s[k], r) - w);
+    }
   }
 }
 
@@ -522,31 +532,35 @@ __device__ __forceinline__ void st_peer_shared(const float* local, uint32_t rank
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 
-constexpr int kRowThreads = 512;
+constexpr int kRowThreads = 256;   // threads that work on the row; one more warp has the list
 constexpr int kMaxRanks = 8;
-constexpr int kRowCtas = 3;   // CTAs per SM that the block kernel is sized for: while one waits for its row, others work
+constexpr int kRowCtas = 3;         // CTAs per SM that its registers allow: while one waits for its row, the others work
 
 template <typename T, int kMode>
-__global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(const DistillParams p, const RowPlan g) {
+__global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kernel(const DistillParams p, const RowPlan g) {
   using PK = Pack16<T>;
   constexpr int kN = PK::kN;
   extern __shared__ __align__(16) uint8_t dsmem[];
-  // [slice][mbarrier 16 B][marks x 2][entries x 2: column, teacher logit, own logit]; rows alternate between the two
+  // [slice][mbarrier 16 B][a bit per column][entries: column, teacher logit, own logit]
   const int words = (g.slice * kN + 2 * kN + 31) / 32;
   const int entries = p.K + 1;
   const PK* row_s = reinterpret_cast<const PK*>(dsmem);
-  uint32_t* bits_s = reinterpret_cast<uint32_t*>(dsmem + static_cast<size_t>(g.slice) * 16 + 16);
-  int* col_all = reinterpret_cast<int*>(bits_s + 2 * words);
-  __shared__ float red[2][5][kRowThreads / 32];
+  uint32_t* bits = reinterpret_cast<uint32_t*>(dsmem + static_cast<size_t>(g.slice) * 16 + 16);
+  int* col_s = reinterpret_cast<int*>(bits + words);
+  float* t_s = reinterpret_cast<float*>(col_s + entries);
+  float* z_s = t_s + entries;
+  __shared__ float red[2][3][kRowThreads / 32];
+  __shared__ float teach[2][3];            // the teacher's reference and sum; whether the row has a label
   __shared__ float peer[2][kMaxRanks][4];  // per CTA of the cluster: maximum, two sums, and its part of the loss
-  __shared__ int twice[2];    // some column occurs more than once
   __shared__ int wait_failed;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x, nwarps = nthreads >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int nthreads = blockDim.x - 32, nwarps = nthreads >> 5;  // those that work on the row
+  const bool list_warp = warp == nwarps;  // stages the row's list, sums the teacher, corrects the listed columns
   const uint32_t rank = g.ranks > 1 ? cluster_rank() : 0;
   const int64_t first_row = g.ranks > 1 ? cluster_index() : blockIdx.x, row_step = g.ranks > 1 ? cluster_count() : gridDim.x;
   const uint32_t buf = sm100::smem_addr(dsmem), bar = buf + static_cast<uint32_t>(g.slice) * 16;
   const bool hard = p.labels != nullptr && p.alpha > 0.0f;
-  const Exps<kMode> x{kLog2e / p.temperature, kLog2e, g.squarings};
+  const Exps<kMode> x{p.cT, kLog2e, g.squarings};
   const int p0 = static_cast<int>(rank) * g.slice;
   const int C = static_cast<int>(p.C);
 
@@ -562,33 +576,38 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
       sm100::bulk_copy_g2s(buf, z + head + static_cast<int64_t>(p0) * kN, static_cast<uint32_t>(n) * 16, bar);
     }
   };
-  // what a thread reads of a row from global memory itself: entry `tid` of its list, and an element outside the packets
-  // (rank 0 has those). Asked for one row ahead.
-  auto list_id = [&](int64_t row, int k) { return k < p.K ? __ldg(p.ids + row * p.K + k) : hard ? __ldg(p.labels + row) : -1; };
+  // What threads read of a row from global memory themselves is asked for one row ahead: the list warp's first kAhead
+  // entries per lane, and (warp 0 of rank 0) the elements outside the packets.
+  constexpr int kAhead = 2;
+  auto list_id = [&](int64_t row, int k) { return k < p.K ? __ldg(p.ids + row * p.K + k) : hard && k == p.K ? __ldg(p.labels + row) : -1; };
   auto list_t = [&](int64_t row, int k) { return k < p.K ? teacher_at(p, row * p.K + k) : 0.0f; };
+  int ahead_id[kAhead];
+  float ahead_t[kAhead], ahead_edge = -INFINITY;
   auto edge_of = [&](int64_t row) {
     const int head = head_elements(static_cast<const T*>(p.z) + row * p.ldz, p.C), tail0 = head + (C - head) / kN * kN;
-    const int edges = rank == 0 ? head + C - tail0 : 0;
-    return tid < edges ? (tid < head ? tid : tail0 + tid - head) : -1;
+    return tid < head + C - tail0 ? (tid < head ? tid : tail0 + tid - head) : -1;
   };
-  auto edge_value = [&](int64_t row, int col) {
-    return col >= 0 ? Cvt<T>::to_f(static_cast<const T*>(p.z)[row * p.ldz + col]) : -INFINITY;
+  auto look_ahead = [&](int64_t row) {
+    if (list_warp) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) ahead_id[i] = list_id(row, lane + 32 * i), ahead_t[i] = list_t(row, lane + 32 * i);
+    }
+    if (warp == 0 && rank == 0) {
+      const int col = edge_of(row);
+      ahead_edge = col >= 0 ? Cvt<T>::to_f(static_cast<const T*>(p.z)[row * p.ldz + col]) : -INFINITY;
+    }
   };
 
   if (tid == 0) {
     sm100::mbar_init(bar, 1);
     sm100::mbar_init_fence();
     wait_failed = 0;
-    twice[0] = twice[1] = 0;
   }
-  for (int i = tid; i < 2 * words; i += nthreads) bits_s[i] = 0u;
+  for (int i = tid; i < words; i += blockDim.x) bits[i] = 0u;
   __syncthreads();
-  int my_id = -1;
-  float my_t = 0.0f, my_edge = -INFINITY;
   if (first_row < p.B) {
     if (tid == 0) fetch(first_row);
-    if (tid < entries) my_id = list_id(first_row, tid), my_t = list_t(first_row, tid);
-    my_edge = edge_value(first_row, edge_of(first_row));
+    look_ahead(first_row);
   }
   bool piped = true;  // false once a copy did not arrive: the remaining rows run on what the buffer holds
   uint32_t phase = 0;
@@ -599,12 +618,9 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
     const T* z = static_cast<const T*>(p.z) + row * p.ldz;
     const int head = head_elements(z, p.C), pn = packets_of(head);
     const int tail0 = head + (C - head) / kN * kN;
-    const int edge_col = edge_of(row);
-    const float fe = my_edge;
-    uint32_t* bits = bits_s + par * words;
-    int* col_s = col_all + par * 3 * entries;
-    float* t_s = reinterpret_cast<float*>(col_s + entries);
-    float* z_s = t_s + entries;
+    const int edge_col = warp == 0 && rank == 0 ? edge_of(row) : -1;
+    const float fe = ahead_edge;
+    bool twice = false;  // list warp: some column occurs more than once
     // the place of a column among this CTA's elements, -1 for another CTA's column
     auto place = [&](int col) {
       if (col < 0) return -1;
@@ -613,86 +629,68 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
       const int at = col - head - p0 * kN;
       return at >= 0 && at < pn * kN ? at : -1;
     };
-    // the row's list: every CTA of a cluster has all of it, marks its own columns and sums the teacher's weights
-    float nt = -INFINITY, st = 0.0f;
-    for (int k = tid; k < entries; k += nthreads) {
-      const int id = k == tid ? my_id : list_id(row, k);
-      const float t = k == tid ? my_t : list_t(row, k);
-      const int col = id >= 0 && id < C ? id : -1;
-      col_s[k] = col;
-      t_s[k] = t;
-      if (col >= 0 && k < p.K) teacher_add(t, x.cT, nt, st);
-      const int at = place(col);
-      if (p.dz && at >= 0 && (atomicOr(bits + (at >> 5), 1u << (at & 31)) & (1u << (at & 31)))) twice[par] = 1;
+    if (list_warp) {
+      // The row's list: every CTA of a cluster has all of it, sums the teacher's weights and marks its own columns.
+      float nt = -INFINITY;
+      auto stage = [&](int k, int id, float t) {
+        const int col = id >= 0 && id < C ? id : -1, at = place(col);
+        col_s[k] = col, t_s[k] = t;
+        if (col >= 0 && k < p.K) nt = fmaxf(nt, t * p.cT);
+        if (p.dz && at >= 0 && (atomicOr(bits + (at >> 5), 1u << (at & 31)) & (1u << (at & 31)))) twice = true;
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (lane + 32 * i < entries) stage(lane + 32 * i, ahead_id[i], ahead_t[i]);
+      for (int k = lane + 32 * kAhead; k < entries; k += 32) stage(k, list_id(row, k), list_t(row, k));
+      nt = warp_max(nt);
+      if (nt == -INFINITY) nt = 0.0f;
+      __syncwarp();
+      float st = 0.0f;
+      for (int k = lane; k < p.K; k += 32)
+        if (col_s[k] >= 0) st += ex2(fmaf(t_s[k], p.cT, -nt));
+      st = warp_sum(st);
+      if (lane == 0) teach[par][0] = nt, teach[par][1] = st, teach[par][2] = col_s[p.K] >= 0 ? 1.0f : 0.0f;
     }
     if (pn > 0 && piped) {
       if (!sm100::mbar_wait_bounded(bar, phase, rowk::kRowWaitBudgetNs)) wait_failed = 1;
       phase ^= 1u;
     }
-    for (int k = tid; k < entries; k += nthreads) {
-      const int col = col_s[k], at = place(col);
-      if (at >= 0) z_s[k] = at < g.slice * kN ? Cvt<T>::to_f(reinterpret_cast<const T*>(dsmem)[at]) : Cvt<T>::to_f(z[col]);
-    }
-    // Maximum and sums in one pass, kGroup packets at a time: a larger maximum rescales the sums so far, which after the
-    // first groups hardly happens.
-    constexpr int kGroup = 2;
-    float m = -INFINITY, n = 0.0f, n1 = 0.0f;
-    uint64_t s2 = pair(0.0f, 0.0f), s12 = s2;
-    auto raise = [&](float to) {
-      if (to > m) {
-        const float nn = __fmul_rn(to, x.cT), nn1 = x.n1_of(to);
-        const float k = m == -INFINITY ? 0.0f : rescale(n, nn), k1 = m == -INFINITY ? 0.0f : rescale(n1, nn1);
-        s2 = mul2(s2, pair(k, k));
-        if constexpr (kMode != kOneExp) s12 = mul2(s12, pair(k1, k1));
-        m = to, n = nn, n1 = nn1;
-      }
-    };
-    if (edge_col >= 0) {
-      raise(fe);
-      x.add(pair(fe, -INFINITY), n, n1, s2, s12);
-    }
-    for (int pi = tid; pi < pn; pi += kGroup * nthreads) {
-      PK v[kGroup];
-      v[0] = row_s[pi];
-      const bool two = pi + nthreads < pn;
-      if (two) v[1] = row_s[pi + nthreads];
-      const float a = max_of(v[0]);
-      raise(two ? fmaxf(a, max_of(v[1])) : a);
-#pragma unroll
-      for (int q = 0; q < kGroup; ++q)
-        if (q == 0 || two) {
-          uint64_t f[kN / 2];
-          unpack_pairs<T>(v[q], f);
-#pragma unroll
-          for (int e = 0; e < kN / 2; ++e) x.add(f[e], n, n1, s2, s12);
-        }
-    }
+    float m = edge_col >= 0 ? fe : -INFINITY;
     RowStats r;
-    {
-      const float mw = warp_max(m), ntw = warp_max(nt);
-      const float nw = mw == -INFINITY ? 0.0f : __fmul_rn(mw, x.cT), nw1 = mw == -INFINITY ? 0.0f : x.n1_of(mw);
+    if (!list_warp) {
+      // Maximum first: its pass takes three instructions for eight 16-bit logits.
+#pragma unroll 4
+      for (int pi = tid; pi < pn; pi += nthreads) m = fmaxf(m, max_of(row_s[pi]));
+      m = warp_max(m);
+      const float ref = m == -INFINITY ? 0.0f : m;
+      const float n = __fmul_rn(ref, p.cT), n1 = x.n1_of(ref);
+      uint64_t s2 = pair(0.0f, 0.0f), s12 = s2;
+      if (warp == 0 && rank == 0) x.add(pair(edge_col >= 0 ? fe : -INFINITY, -INFINITY), n, n1, s2, s12);
+#pragma unroll 4
+      for (int pi = tid; pi < pn; pi += nthreads) {
+        uint64_t f[kN / 2];
+        unpack_pairs<T>(row_s[pi], f);
+#pragma unroll
+        for (int e = 0; e < kN / 2; ++e) x.add(f[e], n, n1, s2, s12);
+      }
       const float2 a = split(s2), b = split(s12);
-      const float s = warp_sum((a.x + a.y) * (m == -INFINITY ? 1.0f : rescale(n, nw)));  // nothing added yet: 0, or NaN
-      const float s1 = kMode == kOneExp ? 0.0f : warp_sum((b.x + b.y) * (m == -INFINITY ? 1.0f : rescale(n1, nw1)));
-      st = warp_sum(nt == -INFINITY ? st : st * rescale(nt, ntw));
-      if (lane == 0) {
-        red[par][0][warp] = mw;
-        red[par][1][warp] = s;
-        red[par][2][warp] = s1;
-        red[par][3][warp] = ntw;
-        red[par][4][warp] = st;
+      const float s = warp_sum(a.x + a.y), s1 = kMode == kOneExp ? 0.0f : warp_sum(b.x + b.y);
+      if (lane == 0) red[par][0][warp] = m, red[par][1][warp] = s, red[par][2][warp] = s1;
+    } else {  // the list's own logits, of this CTA's columns
+      for (int k = lane; k < entries; k += 32) {
+        const int col = col_s[k], at = place(col);
+        if (at >= 0) z_s[k] = at < g.slice * kN ? Cvt<T>::to_f(reinterpret_cast<const T*>(dsmem)[at]) : Cvt<T>::to_f(z[col]);
       }
     }
     __syncthreads();
     {
       // every warp folds the warps' parts for itself, in the same order
       const bool in = lane < nwarps;
-      const float a = in ? red[par][0][lane] : -INFINITY, at = in ? red[par][3][lane] : -INFINITY;
+      const float a = in ? red[par][0][lane] : -INFINITY;
       m = warp_max(a);
-      r.nt = warp_max(at);
-      r.S = warp_sum(in ? red[par][1][lane] * (a == m ? 1.0f : ex2(__fmul_rn(a, x.cT) - __fmul_rn(m, x.cT))) : 0.0f);
+      r.S = warp_sum(in ? red[par][1][lane] * (a == m ? 1.0f : ex2(__fmul_rn(a, p.cT) - __fmul_rn(m, p.cT))) : 0.0f);
       r.S1 = kMode == kOneExp ? r.S : warp_sum(in ? red[par][2][lane] * (a == m ? 1.0f : ex2(x.n1_of(a) - x.n1_of(m))) : 0.0f);
-      r.St = warp_sum(in ? red[par][4][lane] * rescale(at, r.nt) : 0.0f);
+      r.nt = teach[par][0], r.St = teach[par][1];
     }
     if (g.ranks > 1) {
       if (warp == 0 && lane < g.ranks) {
@@ -707,7 +705,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
       r.S = r.S1 = 0.0f;
       for (int k = 0; k < g.ranks; ++k) {
         const float pm = peer[par][k][0];
-        r.S += peer[par][k][1] * (pm == a ? 1.0f : ex2(__fmul_rn(pm, x.cT) - __fmul_rn(a, x.cT)));
+        r.S += peer[par][k][1] * (pm == a ? 1.0f : ex2(__fmul_rn(pm, p.cT) - __fmul_rn(a, p.cT)));
         r.S1 += peer[par][k][2] * (pm == a ? 1.0f : ex2(x.n1_of(pm) - x.n1_of(a)));
       }
       m = a;
@@ -719,18 +717,18 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
     }
     {
       const float ref = m == -INFINITY ? 0.0f : m;
-      r.n = __fmul_rn(ref, x.cT);
+      r.n = __fmul_rn(ref, p.cT);
       r.n1 = x.n1_of(ref);
     }
-    finish_stats(p, kMode, hard && col_s[p.K] >= 0, r);
+    finish_stats<kMode>(p, teach[par][2] != 0.0f, r);
     const bool dead = !r.some && !r.known;
     T* out = static_cast<T*>(p.dz) + row * p.lddz;
-    if (p.dz) {
+    if (p.dz && !list_warp) {
       PK* packets = reinterpret_cast<PK*>(out + head) + p0;
       if (dead) {  // neither term: zeros, whatever the logits hold
         for (int pi = tid; pi < pn; pi += nthreads) st_stream(packets + pi, zero_packet<T>());
       } else {
-#pragma unroll 2
+#pragma unroll 4
         for (int pi = tid; pi < pn; pi += nthreads) {
           uint64_t f[kN / 2];
           unpack_pairs<T>(row_s[pi], f);
@@ -740,7 +738,6 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
         }
       }
       if (edge_col >= 0) out[edge_col] = Cvt<T>::from_f(dead ? 0.0f : x.grad1(fe, r));
-      if (tid == 0) twice[par ^ 1] = 0;  // last read one row ago, next set behind this barrier
     }
     __syncthreads();  // the buffer is free; the corrections below come behind the row's stores
     if (wait_failed) piped = false;
@@ -750,28 +747,20 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
         sm100::fence_generic_to_async_smem();
         fetch(next);
       }
-      if (tid < entries) my_id = list_id(next, tid), my_t = list_t(next, tid);
-      my_edge = edge_value(next, edge_of(next));
-    }
-    if (warp == nwarps - 1) {  // this CTA's part of the loss: its own columns' logits
-      float own = 0.0f;
-      if (r.some) {
-        for (int k = lane; k < p.K; k += 32)
-          if (place(col_s[k]) >= 0) own += cross_term(r, x.cT, t_s[k], z_s[k]);
-        own = (1.0f - p.alpha) * p.temperature * p.temperature * warp_sum(own);
-      }
-      if (lane == 0) {
-        if (r.known && place(col_s[p.K]) >= 0) own += label_term(p, r, z_s[p.K], x.c1);
-        if (g.ranks > 1) st_peer_shared(&peer[par][rank][3], 0, own);
-        else p.loss[row] = loss_of_sums(p, r) + own;
-      }
+      look_ahead(next);
     }
     if (rank == 0 && tid == 0 && g.ranks > 1) owed = row, owed_base = loss_of_sums(p, r);
-    if (p.dz) {
-      const bool dup = twice[par] != 0;
-      for (int k = tid; k < entries; k += nthreads) {
+    if (list_warp) {
+      // this CTA's part of the loss, and the corrections of its columns: equal columns are corrected once, by their first
+      // entry, for the sum of their weights in the list's order
+      const bool dup = __any_sync(0xffffffffu, twice);
+      auto weight = [&](int j) { return j == p.K ? p.grad_hard : p.grad_soft * target(p, r, t_s[j]); };
+      float own = 0.0f;
+      for (int k = lane; k < entries; k += 32) {
         const int col = col_s[k], at = place(col);
         if (at < 0) continue;
+        if (k < p.K && r.some) own += cross_term(p, r, t_s[k], z_s[k]);
+        if (!p.dz) continue;
         bits[at >> 5] = 0u;  // this row's marks go
         float w = 0.0f;
         bool first = !dead;
@@ -779,13 +768,20 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) distill_block_kernel(co
           for (int j = 0; j < entries; ++j)
             if (col_s[j] == col) {
               if (j < k) first = false;
-              w += entry_weight(p, r, x.cT, j, t_s[j]);
+              w += weight(j);
             }
         } else {
-          w = entry_weight(p, r, x.cT, k, t_s[k]);
+          w = weight(k);
         }
         if (first) out[col] = Cvt<T>::from_f(x.grad1(z_s[k], r) - w);
       }
+      own = loss_of_list(p, warp_sum(own));
+      if (lane == 0) {
+        if (r.known && place(col_s[p.K]) >= 0) own += loss_of_label(p, r, z_s[p.K], x.c1);
+        if (g.ranks > 1) st_peer_shared(&peer[par][rank][3], 0, own);
+        else p.loss[row] = loss_of_sums(p, r) + own;
+      }
+      __syncwarp();  // the list is the next row's from here on
     }
   }
   if (g.ranks > 1) {
@@ -820,25 +816,26 @@ bool plan_rows(const DistillParams& p, RowPlan* out) {
     g.packets = 1;
     while (g.packets < per) g.packets *= 2;
     g.slice = static_cast<int>(packets);
-    g.smem = kRowsPerBlock * (static_cast<size_t>((p.C + 31) / 32) * 4 + list);
+    g.smem = p.K < 32 ? 0 : kRowsPerBlock * (static_cast<size_t>((p.C + 31) / 32) * 4 + list);
     *out = g;
     return true;
   }
   auto bytes = [&](int64_t slice) {
-    return static_cast<size_t>(slice) * 16 + 16 + 2 * static_cast<size_t>((slice * kN + 2 * kN + 31) / 32) * 4 + 2 * list;
+    return static_cast<size_t>(slice) * 16 + 16 + static_cast<size_t>((slice * kN + 2 * kN + 31) / 32) * 4 + list;
   };
-  constexpr size_t kShare = (227 * 1024) / kRowCtas - 2048;  // an SM's shared memory over its CTAs, less the static part
-  int limit_ranks = kMaxRanks;
-  while (g.ranks < limit_ranks && bytes((packets + g.ranks - 1) / g.ranks) > kShare) g.ranks *= 2;
-  if (const char* e = std::getenv("AICF_DISTILL_RANKS")) { const int v = std::atoi(e); if (v > 0) g.ranks = v; }
+  // The fewest CTAs per row of which an SM still holds two: one alone would leave the SM idle while it waits for its row
+  // (8192 x 32000 f32 in 374 us as two slices per row, 528 as one), and every doubling costs a cluster barrier more than it
+  // hides (4096 x 100003 bf16: 375 us as two slices, 412 as four; 8192 x 32000 bf16: 203 as one, 303 as two).
+  constexpr size_t kShare = (227 * 1024) / 2 - 2048;  // half an SM's shared memory, less the static part
+  while (g.ranks < kMaxRanks && bytes((packets + g.ranks - 1) / g.ranks) > kShare) g.ranks *= 2;
   const int64_t slice = (packets + g.ranks - 1) / g.ranks;
   g.smem = bytes(slice);
   if (g.smem > 200 * 1024) return false;
   g.slice = static_cast<int>(slice);
-  int grow = 4; 
-  if (const char* e = std::getenv("AICF_DISTILL_GROW")) grow = std::atoi(e);
-  g.threads = 128;
-  while (g.threads < kRowThreads && static_cast<int64_t>(g.threads) * grow < slice) g.threads *= 2;
+  // Sixteen packets per thread before the block grows: what a thread does per row besides its packets (folding the warps'
+  // parts, the factors) costs as much as eight of them (16384 x 8192 bf16: 216 / 166 / 152 us at 4 / 8 / 16).
+  g.threads = 32;
+  while (g.threads < kRowThreads && static_cast<int64_t>(g.threads) * 16 < slice) g.threads *= 2;
   *out = g;
   return true;
 }
@@ -857,10 +854,11 @@ Status launch_block_rows(const DistillParams& p, const RowPlan& g, cudaStream_t 
   attr[0].val.clusterDim.x = static_cast<unsigned>(g.ranks);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  // registers allow kRowCtas blocks of kRowThreads threads
-  int resident = rowk::row_pipe_blocks_per_sm(g.threads, g.smem + 1024);
-  if (resident > kRowCtas * kRowThreads / g.threads) resident = kRowCtas * kRowThreads / g.threads;
-  cfg.blockDim = dim3(static_cast<unsigned>(g.threads));
+  // registers allow kRowCtas blocks of kRowThreads + 32 threads
+  const int threads = g.threads + 32;
+  int resident = rowk::row_pipe_blocks_per_sm(threads, g.smem + 1024);
+  if (resident > kRowCtas * (kRowThreads + 32) / threads) resident = kRowCtas * (kRowThreads + 32) / threads;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = g.smem;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -894,9 +892,9 @@ Status launch_block_rows(const DistillParams& p, const RowPlan& g, cudaStream_t 
   }
   return launch_status();
 }
-template <typename T, int kPk, int kMode>
-Status launch_warp_rows(const DistillParams& p, const RowPlan& g, cudaStream_t stream) {
-  auto kernel = distill_warp_kernel<T, kPk, kMode>;
+template <typename T, int kPk, int kMode, bool kOneEach>
+Status launch_warp_list(const DistillParams& p, const RowPlan& g, cudaStream_t stream) {
+  auto kernel = distill_warp_kernel<T, kPk, kMode, kOneEach>;
   static PerDeviceOnce opt_in;
   if (!opt_in.run([&] { return rowk::allow_smem(kernel, 110 * 1024); })) {
     cudaGetLastError();
@@ -906,6 +904,10 @@ Status launch_warp_rows(const DistillParams& p, const RowPlan& g, cudaStream_t s
   if (blocks > 0x7fffffff) return Status::InvalidArgument;
   kernel<<<static_cast<unsigned>(blocks), 32 * kRowsPerBlock, g.smem, stream>>>(p, g);
   return launch_status();
+}
+template <typename T, int kPk, int kMode>
+Status launch_warp_rows(const DistillParams& p, const RowPlan& g, cudaStream_t stream) {
+  return p.K < 32 ? launch_warp_list<T, kPk, kMode, true>(p, g, stream) : launch_warp_list<T, kPk, kMode, false>(p, g, stream);
 }
 template <typename T, int kMode>
 Status launch_mode(const DistillParams& p, const RowPlan& g, cudaStream_t stream) {
@@ -957,6 +959,10 @@ bool distill_check(DType dt, const TensorDesc* in, int ni, const TensorDesc* out
   } else if (p.alpha > 0.0f) {
     return false;  // a label term without labels
   }
+  p.cT = kLog2e / p.temperature;
+  p.grad_soft = p.scale * (1.0f - p.alpha) * p.temperature;
+  p.grad_hard = p.scale * p.alpha;
+  p.loss_soft = (1.0f - p.alpha) * p.temperature * p.temperature;
   p.z = Z.data, p.ldz = p.B == 1 ? p.C : Z.stride[0];
   if (no == 2) p.dz = out[0].data, p.lddz = p.B == 1 ? p.C : out[0].stride[0];
   p.ids = static_cast<const int32_t*>(I.data);
