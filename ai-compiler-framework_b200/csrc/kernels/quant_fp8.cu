@@ -8,12 +8,20 @@
 //           [q, s, q', s']   the row form and the column form of the same matrix, x read once
 //
 // With F the format's largest value (448, 57344) and amax the block's largest magnitude, but at least 2^-100:
-//   s = amax / F,   q = round_to_nearest_even(x * (F / amax)),   x ~ q * s
-// (both quotients and the product in fp32, one rounding each; the lower limit keeps F / amax finite, and a block of
-// zeros gets zeros). A NaN or an infinity in a block makes its scale NaN or infinite and its own value NaN.
+//   s = amax / F rounded to fp32,   q = the format's value nearest to x F / amax (ties to even),   x ~ q * s
+// q is rounded once, from the exact quotient; the lower limit keeps F / amax finite, and a block of zeros gets zeros. A NaN or
+// an infinity makes its block's scale NaN or infinite and its values NaN.
 //
-// A block of 256 threads owns one 128 x 128 tile and keeps it in registers (8 rows of 8 columns per thread), so all
-// three forms come from one read.
+// A block of threads owns one 128 x 128 tile and keeps it in registers as it was read, eight columns of kRows rows per
+// thread, so all forms come from one read. HBM bounds it (4 bytes per bf16 value for both forms), with instruction issue close
+// behind: about 17 instructions per value for two forms, hence packed 16-bit maxima, one division per row and column of the
+// tile, and the exact rounding below without a branch in the usual case.
+//
+// Rounding. p = x inv + x inv_lo with inv + inv_lo = F / amax to 2^-48 is x F / amax rounded to fp32. Rounding p to eight bits
+// gives the right value unless p is exactly half way between two of them, where the quotient itself may lie to either side:
+// such a p (one in 2^20 fp32 values) is held against the quotient by the sign of x F - p amax. With 16-bit inputs it cannot
+// happen: x F / amax = X F / A with X and A of at most 11 bits differs from a half-way point of 5 bits by 2^-16 of itself or
+// not at all.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -23,11 +31,7 @@ namespace aicf::cuda {
 namespace {
 
 constexpr int kBlk = 128;
-constexpr int kQThreads = 256;
-constexpr int kColsPerThread = 8;
-constexpr int kLanesPerRow = kBlk / kColsPerThread;        // 16 threads cover a row of the tile
-constexpr int kRowsPerPass = kQThreads / kLanesPerRow;     // 16
-constexpr int kPasses = kBlk / kRowsPerPass;               // 8
+constexpr int kLanesPerRow = 16;                           // eight columns each
 constexpr float kTiny = 7.888609052210118e-31f;            // 2^-100
 
 enum QuantForms : int { kRowForm = 1, kColForm = 2, kTileForm = 4 };
@@ -48,135 +52,274 @@ struct QuantParams {
   QuantOut row, col;     // the tile form uses `row`
 };
 
-// |a| and b, NaN wins
-__device__ __forceinline__ float amax_of(float b, float a) {
-  float r;
-  asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %1;\n\tmax.NaN.f32 %0, t, %2;\n\t}" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t to_fp8x2(float a, float b, int e5m2) {
-  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, e5m2 ? __NV_E5M2 : __NV_E4M3));
-}
 __device__ __forceinline__ float top_of(int e5m2) { return e5m2 ? 57344.0f : 448.0f; }
 
+// Magnitudes as integers: with the sign bit cleared, the order of the bit patterns is the order of the magnitudes, infinities
+// and NaNs above everything. 16-bit types go two to a word.
+template <typename T> struct Mag {
+  static constexpr int kWords = 8;   // words that hold eight values
+  __device__ __forceinline__ static uint32_t clear(uint32_t w) { return w & 0x7FFFFFFFu; }
+  __device__ __forceinline__ static uint32_t max(uint32_t a, uint32_t b) { return a > b ? a : b; }
+};
+template <typename T> struct Mag16 {
+  static constexpr int kWords = 4;
+  __device__ __forceinline__ static uint32_t clear(uint32_t w) { return w & 0x7FFF7FFFu; }
+  __device__ __forceinline__ static uint32_t max(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+};
+template <> struct Mag<__half> : Mag16<__half> {};
+template <> struct Mag<__nv_bfloat16> : Mag16<__nv_bfloat16> {};
+// the value of a magnitude pattern (low half of the word for the 16-bit types)
+template <typename T> __device__ __forceinline__ float mag_value(uint32_t w) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(w);
+  } else {
+    const uint16_t h = static_cast<uint16_t>(w);
+    T t;
+    memcpy(&t, &h, 2);
+    return Cvt<T>::to_f(t);
+  }
+}
+
+// What a block's largest magnitude comes down to.
+struct Factor {
+  float amax, inv, lo;  // F / amax = inv + lo
+  __device__ __forceinline__ Factor() {}
+  __device__ __forceinline__ Factor(float a, float top) {
+    amax = a < kTiny ? kTiny : a;  // a NaN stays
+    inv = top / amax;
+    lo = fmaf(-amax, inv, top) * (inv / top);
+  }
+};
+
+// Eight values as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int valid, float (&f)[8]) {
+__device__ __forceinline__ void load8(const T* p, bool vec, int valid, uint32_t (&w)[Mag<T>::kWords]) {
   if (vec && valid >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      float a[4], b[4];
-      unpack16(ld_stream(reinterpret_cast<const Pack16<T>*>(p)), a);
-      unpack16(ld_stream(reinterpret_cast<const Pack16<T>*>(p) + 1), b);
+    const int4* src = reinterpret_cast<const int4*>(p);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
-    } else {
-      unpack16(ld_stream(reinterpret_cast<const Pack16<T>*>(p)), f);
+    for (int i = 0; i < Mag<T>::kWords / 4; ++i) {
+      const int4 t = __ldcs(src + i);
+      w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = e < valid ? Cvt<T>::to_f(p[e]) : 0.0f;
+    for (int i = 0; i < Mag<T>::kWords; ++i) w[i] = 0u;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < valid) w[e] = reinterpret_cast<const uint32_t*>(p)[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < valid) w[e >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
+    }
   }
 }
-
-__device__ __forceinline__ void store8(const QuantOut& o, int64_t row, int64_t col, int valid, const float (&f)[8], const float (&inv)[8]) {
-  if (valid <= 0) return;
-  uint32_t h[4];
+template <typename T>
+__device__ __forceinline__ void values8(const uint32_t (&w)[Mag<T>::kWords], float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) h[e] = to_fp8x2(f[2 * e] * inv[2 * e], f[2 * e + 1] * inv[2 * e + 1], o.e5m2);
-  uint8_t* dst = o.q + row * o.ld + col;
-  if (o.vec && valid >= 8) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(w[e]);
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < valid) dst[e] = static_cast<uint8_t>(h[e >> 1] >> (8 * (e & 1)));
+    Pack16<T> p;
+    *reinterpret_cast<uint4*>(&p) = make_uint4(w[0], w[1], w[2], w[3]);
+    unpack16(p, f);
   }
 }
 
-template <typename T, int kForms>
-__global__ void __launch_bounds__(kQThreads) quant_fp8_kernel(const QuantParams p) {
-  __shared__ float part[kQThreads / 32][kBlk];
-  const int cg = threadIdx.x % kLanesPerRow, rl = threadIdx.x / kLanesPerRow;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t tm = blockIdx.x / p.tiles_n, tn = blockIdx.x % p.tiles_n;
-  const int64_t row0 = tm * kBlk + rl, col = tn * kBlk + cg * kColsPerThread;
-  const int valid = p.N - col >= 8 ? 8 : static_cast<int>(p.N - col);  // columns of this thread inside the matrix
-  float v[kPasses][8];
+// A p that lies exactly between two values of the format moves one step towards the exact quotient x F / amax. The sign of
+// x F - p amax comes from both products' heads and errors: the heads are equal to a few units, so their difference is exact.
+__device__ __forceinline__ float off_the_tie(float p, float x, float amax, float top) {
+  const float have = p * amax, want = x * top;
+  const float d = (want - have) + (fmaf(x, top, -want) - fmaf(p, amax, -have));
+  const float towards = p < 0.0f ? -d : d;  // > 0: the quotient's magnitude is larger
+  const int step = towards > 0.0f ? 1 : towards < 0.0f ? -1 : 0;
+  return __int_as_float(__float_as_int(p) + step);
+}
+
+// Eight values to eight bytes. `amax(e)` is asked for in the rare case only.
+template <typename T, typename Inv, typename Lo, typename Amax>
+__device__ __forceinline__ uint2 quant8(const float (&x)[8], int e5m2, Inv inv, Lo lo, Amax amax) {
+  float p[8];
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int64_t row = row0 + i * kRowsPerPass;
-    load8(static_cast<const T*>(p.x) + row * p.ldx + col, p.vec_in != 0, row < p.M ? valid : 0, v[i]);
-  }
-  if constexpr ((kForms & kRowForm) != 0) {
-    const float top = top_of(p.row.e5m2);
+  for (int e = 0; e < 8; ++e) p[e] = fmaf(x[e], inv(e), x[e] * lo(e));
+  if constexpr (sizeof(T) == 4) {
+    const float least = e5m2 ? 6.103515625e-05f : 0.015625f;  // smallest normal value
+    const uint32_t half = e5m2 ? 0x100000u : 0x80000u, mask = 2u * half - 1u;
+    bool tie = false;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int64_t row = row0 + i * kRowsPerPass;
-      float a = kTiny;
+    for (int e = 0; e < 8; ++e) {
+      // a value below the normal range is lifted into it, where its half steps have the same bit pattern as everybody's (where
+      // the lifting rounds, a tie may be seen that is none: it is looked at again)
+      float y = fabsf(p[e]);
+      asm("{\n\t.reg .pred q;\n\tsetp.lt.f32 q, %0, %1;\n\t@q add.f32 %0, %0, %1;\n\t}" : "+f"(y) : "f"(least));
+      tie |= (__float_as_uint(y) & mask) == half;
+    }
+    if (__builtin_expect(tie, 0)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a = amax_of(a, v[i][e]);
-#pragma unroll
-      for (int o = kLanesPerRow / 2; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-      const float k = top / a;
-      const float inv[8] = {k, k, k, k, k, k, k, k};
-      if (row < p.M) {
-        store8(p.row, row, col, valid, v[i], inv);
-        if (cg == 0) p.row.s[row * p.row.s0 + tn * p.row.s1] = a / top;
+      for (int e = 0; e < 8; ++e) {
+        const float a = fabsf(p[e]), y = a < least ? __fadd_rn(a, least) : a;
+        if ((__float_as_uint(y) & mask) == half && (a >= least || __fadd_rn(y, -least) == a))
+          p[e] = off_the_tie(p[e], x[e], amax(e), top_of(e5m2));
       }
     }
   }
-  if constexpr ((kForms & kColForm) != 0) {
-    const float top = top_of(p.col.e5m2);
-    float a[8];
+  uint32_t h[4];
+  if (e5m2) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      a[e] = kTiny;
+    for (int e = 0; e < 4; ++e) h[e] = __nv_cvt_float2_to_fp8x2(make_float2(p[2 * e], p[2 * e + 1]), __NV_SATFINITE, __NV_E5M2);
+  } else {
 #pragma unroll
-      for (int i = 0; i < kPasses; ++i) a[e] = amax_of(a[e], v[i][e]);
-      a[e] = max_nan(a[e], __shfl_xor_sync(0xffffffffu, a[e], 16));
-      if (lane < 16) part[warp][cg * 8 + e] = a[e];
+    for (int e = 0; e < 4; ++e) h[e] = __nv_cvt_float2_to_fp8x2(make_float2(p[2 * e], p[2 * e + 1]), __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+__device__ __forceinline__ void store8(const QuantOut& o, int64_t row, int64_t col, int valid, uint2 b) {
+  uint8_t* dst = o.q + row * o.ld + col;
+  if (o.vec && valid >= 8) {
+    *reinterpret_cast<uint2*>(dst) = b;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < valid) dst[e] = static_cast<uint8_t>((e < 4 ? b.x : b.y) >> (8 * (e & 3)));
+  }
+}
+
+// Rows per thread: 32 registers hold eight rows of a 16-bit type or four of fp32.
+template <typename T> struct Shape {
+  static constexpr int kRows = sizeof(T) == 4 ? 4 : 8;
+  static constexpr int kThreads = kBlk / kRows * kLanesPerRow;  // 512 or 256
+  static constexpr int kWarps = kThreads / 32;
+  static constexpr int kRowStep = kThreads / kLanesPerRow;      // rows between a thread's rows
+};
+
+template <typename T, int kForms>
+__global__ void __launch_bounds__(Shape<T>::kThreads, sizeof(T) == 4 ? 2 : kForms == (kRowForm | kColForm) ? 3 : 4) quant_fp8_kernel(const QuantParams p) {
+  using G = Mag<T>;
+  constexpr int kRows = Shape<T>::kRows, kWarps = Shape<T>::kWarps, kRowStep = Shape<T>::kRowStep, kW = G::kWords;
+  __shared__ uint32_t part[kWarps][kLanesPerRow][kW];  // a warp's maxima of each lane's columns
+  __shared__ float col_inv[kBlk], col_lo[kBlk], col_amax[kBlk], row_amax[kBlk];
+  const int cg = threadIdx.x % kLanesPerRow, rl = threadIdx.x / kLanesPerRow;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t tm = blockIdx.x / p.tiles_n, tn = blockIdx.x % p.tiles_n;
+  const int64_t row0 = tm * kBlk + rl, col = tn * kBlk + cg * 8;
+  const int valid = p.N - col >= 8 ? 8 : p.N > col ? static_cast<int>(p.N - col) : 0;  // columns of this thread inside
+  uint32_t w[kRows][kW];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t row = row0 + i * kRowStep;
+    load8<T>(static_cast<const T*>(p.x) + row * p.ldx + col, p.vec_in != 0, row < p.M ? valid : 0, w[i]);
+  }
+  // ---- columns (and the tile): each lane's eight over its rows, over the two half warps, over the warps
+  if constexpr (kForms != kRowForm) {
+    uint32_t a[kW];
+#pragma unroll
+    for (int k = 0; k < kW; ++k) {
+      a[k] = G::clear(w[0][k]);
+#pragma unroll
+      for (int i = 1; i < kRows; ++i) a[k] = G::max(a[k], G::clear(w[i][k]));
+      a[k] = G::max(a[k], __shfl_xor_sync(0xffffffffu, a[k], 16));
     }
-    __syncthreads();
-    float inv[8];
+    if (lane < 16) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      a[e] = part[0][cg * 8 + e];
-#pragma unroll
-      for (int w = 1; w < kQThreads / 32; ++w) a[e] = max_nan(a[e], part[w][cg * 8 + e]);
-      inv[e] = top / a[e];
-      if (rl == 0 && e < valid) p.col.s[tm * p.col.s0 + (col + e) * p.col.s1] = a[e] / top;
-    }
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int64_t row = row0 + i * kRowsPerPass;
-      if (row < p.M) store8(p.col, row, col, valid, v[i], inv);
+      for (int k = 0; k < kW; k += 4) *reinterpret_cast<uint4*>(&part[warp][cg][k]) = make_uint4(a[k], a[k + 1], a[k + 2], a[k + 3]);
     }
   }
-  if constexpr (kForms == kTileForm) {
-    const float top = top_of(p.row.e5m2);
-    float a = kTiny;
+  // ---- rows: kRows maxima over the sixteen lanes of a row; 16-bit types two rows to a word
+  Factor rf;            // of the row this lane works out: row cg of its kRows
+  if constexpr ((kForms & kRowForm) != 0) {
+    constexpr int kR = sizeof(T) == 4 ? kRows : kRows / 2;
+    uint32_t a[kR];
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i)
+    for (int i = 0; i < kR; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        a[i] = G::clear(w[i][0]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a = amax_of(a, v[i][e]);
+        for (int k = 1; k < kW; ++k) a[i] = G::max(a[i], G::clear(w[i][k]));
+      } else {
+        uint32_t b[2];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-    if (lane == 0) part[0][warp] = a;
-    __syncthreads();
+        for (int h = 0; h < 2; ++h) {
+          b[h] = G::clear(w[2 * i + h][0]);
 #pragma unroll
-    for (int w = 0; w < kQThreads / 32; ++w) a = max_nan(a, part[0][w]);
-    const float k = top / a;
-    const float inv[8] = {k, k, k, k, k, k, k, k};
+          for (int k = 1; k < kW; ++k) b[h] = G::max(b[h], G::clear(w[2 * i + h][k]));
+        }
+        // low halves of both rows side by side, high halves too, then one maximum: row 2i below, row 2i + 1 above
+        a[i] = G::max(__byte_perm(b[0], b[1], 0x5410), __byte_perm(b[0], b[1], 0x7632));
+      }
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int64_t row = row0 + i * kRowsPerPass;
-      if (row < p.M) store8(p.row, row, col, valid, v[i], inv);
+      for (int o = kLanesPerRow / 2; o > 0; o >>= 1) a[i] = G::max(a[i], __shfl_xor_sync(0xffffffffu, a[i], o));
     }
-    if (threadIdx.x == 0) p.row.s[tm * p.row.s0 + tn * p.row.s1] = a / top;
+    uint32_t mine = a[0];
+#pragma unroll
+    for (int i = 1; i < kR; ++i)
+      if ((sizeof(T) == 4 ? cg : cg >> 1) == i) mine = a[i];
+    if (sizeof(T) != 4 && (cg & 1)) mine >>= 16;
+    rf = Factor(mag_value<T>(sizeof(T) == 4 ? mine : mine & 0xFFFFu), top_of(p.row.e5m2));
+    const int64_t row = row0 + cg * kRowStep;
+    if (cg < kRows) {
+      row_amax[rl + cg * kRowStep] = rf.amax;
+      if (row < p.M) p.row.s[row * p.row.s0 + tn * p.row.s1] = rf.amax / top_of(p.row.e5m2);
+    }
+  }
+  Factor tile;
+  if constexpr (kForms != kRowForm) {
+    __syncthreads();
+    if (threadIdx.x < kBlk) {
+      const int k = threadIdx.x % 8, l = threadIdx.x / 8;  // column 8 l + k
+      uint32_t a = 0u;
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) a = G::max(a, sizeof(T) == 4 ? part[v][l][k % kW] : part[v][l][(k >> 1) % kW]);
+      if (sizeof(T) != 4) a = (k & 1) ? a >> 16 : a & 0xFFFFu;
+      if constexpr (kForms == kTileForm) {
+        // the tile: over its columns, which are the first four warps' lanes
+        a = __reduce_max_sync(0xffffffffu, a);
+        if (lane == 0) col_amax[warp] = mag_value<T>(a);
+      } else {
+        const Factor f(mag_value<T>(a), top_of(p.col.e5m2));
+        col_inv[threadIdx.x] = f.inv, col_lo[threadIdx.x] = f.lo, col_amax[threadIdx.x] = f.amax;
+        const int64_t c = tn * kBlk + threadIdx.x;
+        if (c < p.N) p.col.s[tm * p.col.s0 + c * p.col.s1] = f.amax / top_of(p.col.e5m2);
+      }
+    }
+    __syncthreads();
+    if constexpr (kForms == kTileForm) {
+      // the bit patterns again, so that a NaN wins
+      uint32_t a = __float_as_uint(col_amax[0]);
+#pragma unroll
+      for (int v = 1; v < 4; ++v) a = max(a, __float_as_uint(col_amax[v]));
+      tile = Factor(__uint_as_float(a), top_of(p.row.e5m2));
+      if (threadIdx.x == 0) p.row.s[tm * p.row.s0 + tn * p.row.s1] = tile.amax / top_of(p.row.e5m2);
+    }
+  } else {
+    __syncwarp();  // row_amax: written and read within a row's sixteen lanes
+  }
+  float ci[8], cl[8];
+  if constexpr ((kForms & kColForm) != 0) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const float4 a = *reinterpret_cast<const float4*>(&col_inv[cg * 8 + e]), b = *reinterpret_cast<const float4*>(&col_lo[cg * 8 + e]);
+      ci[e] = a.x, ci[e + 1] = a.y, ci[e + 2] = a.z, ci[e + 3] = a.w;
+      cl[e] = b.x, cl[e + 1] = b.y, cl[e + 2] = b.z, cl[e + 3] = b.w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t row = row0 + i * kRowStep;
+    float f[8];
+    values8<T>(w[i], f);
+    float inv = tile.inv, lo = tile.lo;
+    if constexpr ((kForms & kRowForm) != 0) {
+      inv = __shfl_sync(0xffffffffu, rf.inv, (lane & 16) + i);
+      lo = __shfl_sync(0xffffffffu, rf.lo, (lane & 16) + i);
+    }
+    if (row >= p.M || valid == 0) continue;
+    if constexpr ((kForms & (kRowForm | kTileForm)) != 0)
+      store8(p.row, row, col, valid, quant8<T>(f, p.row.e5m2, [&](int) { return inv; }, [&](int) { return lo; },
+                                            [&](int) { return kForms == kTileForm ? tile.amax : row_amax[rl + i * kRowStep]; }));
+    if constexpr ((kForms & kColForm) != 0)
+      store8(p.col, row, col, valid, quant8<T>(f, p.col.e5m2, [&](int e) { return ci[e]; }, [&](int e) { return cl[e]; },
+                                            [&](int e) { return col_amax[cg * 8 + e]; }));
   }
 }
 
@@ -237,10 +380,10 @@ Status quant_run(const QuantParams& p, int forms, cudaStream_t stream) {
   const unsigned grid = static_cast<unsigned>(blocks_of(p.M) * p.tiles_n);
   cudaGetLastError();
   switch (forms) {
-    case kRowForm: quant_fp8_kernel<T, kRowForm><<<grid, kQThreads, 0, stream>>>(p); break;
-    case kColForm: quant_fp8_kernel<T, kColForm><<<grid, kQThreads, 0, stream>>>(p); break;
-    case kTileForm: quant_fp8_kernel<T, kTileForm><<<grid, kQThreads, 0, stream>>>(p); break;
-    default: quant_fp8_kernel<T, (kRowForm | kColForm)><<<grid, kQThreads, 0, stream>>>(p); break;
+    case kRowForm: quant_fp8_kernel<T, kRowForm><<<grid, Shape<T>::kThreads, 0, stream>>>(p); break;
+    case kColForm: quant_fp8_kernel<T, kColForm><<<grid, Shape<T>::kThreads, 0, stream>>>(p); break;
+    case kTileForm: quant_fp8_kernel<T, kTileForm><<<grid, Shape<T>::kThreads, 0, stream>>>(p); break;
+    default: quant_fp8_kernel<T, (kRowForm | kColForm)><<<grid, Shape<T>::kThreads, 0, stream>>>(p); break;
   }
   return launch_status();
 }

@@ -236,8 +236,10 @@ def _spread(s, shape):
 
 
 def quant_fp8(X, form, fmt):
-    """(q, s): per block ('rows' 1x128, 'cols' 128x1, 'tiles' 128x128) amax = max(max|x|, 2^-100), s = amax / F,
-    q = round(x * (F / amax)); both quotients and the product rounded to fp32 whatever the type of X."""
+    """(q, s): per block ('rows' 1x128, 'cols' 128x1, 'tiles' 128x128) amax = max(max|x|, 2^-100), s = amax / F rounded to
+    fp32, q = the value nearest to x F / amax (x F is exact in 64 bits, and the quotient's rounding to 53 bits cannot move it
+    onto or across a tie of the 8-bit format: a tie has 5 significant bits, so x F / amax differs from it by 2^-30 or not at
+    all)."""
     x = np.asarray(X, np.float32)
     M, N = x.shape
     by, bx = (128 if form in ("cols", "tiles") else 1), (128 if form in ("rows", "tiles") else 1)
@@ -247,8 +249,8 @@ def quant_fp8(X, form, fmt):
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
         amax = np.maximum(np.abs(padded.reshape(mb, by, nb, bx)).max(axis=(1, 3)), np.float32(2.0 ** -100))
         top = np.float32(FP8_TOP[fmt])
-        inv = (top / amax).astype(np.float32)
-        return fp8_round(x * _spread(inv, x.shape), fmt), (amax / top).astype(np.float32)
+        q = fp8_round(x.astype(np.float64) * float(top) / _spread(amax.astype(np.float64), x.shape), fmt)
+        return q, (amax / top).astype(np.float32)
 
 
 def dequant_fp8(q, s, dt=np.float64):
