@@ -76,25 +76,66 @@ int dtype_code(const py::handle& dtype) {
   return code;
 }
 
+// Attribute names as interned string objects, made once: looking an attribute up by a C string builds a new string object
+// every time, which was half of the cost of a descriptor. Never released (see dtype_code).
+struct Names {
+  PyObject* data_ptr = PyUnicode_InternFromString("data_ptr");
+  PyObject* is_cuda = PyUnicode_InternFromString("is_cuda");
+  PyObject* shape = PyUnicode_InternFromString("shape");
+  PyObject* stride = PyUnicode_InternFromString("stride");
+  PyObject* dtype = PyUnicode_InternFromString("dtype");
+  PyObject* is_contiguous = PyUnicode_InternFromString("is_contiguous");
+};
+const Names& names() {
+  static const Names* n = new Names();
+  return *n;
+}
+py::object attr(const py::handle& o, PyObject* name) {
+  PyObject* v = PyObject_GetAttr(o.ptr(), name);
+  if (!v) throw py::error_already_set();
+  return py::reinterpret_steal<py::object>(v);
+}
+py::object call(const py::handle& o, PyObject* name) {
+  PyObject* v = PyObject_CallMethodNoArgs(o.ptr(), name);
+  if (!v) throw py::error_already_set();
+  return py::reinterpret_steal<py::object>(v);
+}
+int64_t as_int(PyObject* o) {
+  const long long v = PyLong_CheckExact(o) ? PyLong_AsLongLong(o) : py::handle(o).cast<long long>();
+  if (v == -1 && PyErr_Occurred()) throw py::error_already_set();
+  return v;
+}
+// The sequence as a tuple: the object itself where it is one (torch.Size is).
+py::tuple as_tuple(const py::object& o) {
+  return PyTuple_Check(o.ptr()) ? py::reinterpret_borrow<py::tuple>(o) : py::tuple(o);
+}
+
 void fill_desc(aicf_tensor_desc& d, const py::handle& t, const char* what) {
-  if (t.is_none() || !py::hasattr(t, "data_ptr")) throw std::runtime_error(std::string(what) + ": undefined tensor");
-  if (py::hasattr(t, "is_cuda") && !t.attr("is_cuda").cast<bool>())
-    throw std::runtime_error(std::string(what) + ": must be CUDA tensor. got: device=cpu dtype=" + std::string(py::str(t.attr("dtype"))));
-  const py::tuple shape = py::tuple(t.attr("shape"));
+  const Names& n = names();
+  if (t.is_none() || !PyObject_HasAttr(t.ptr(), n.data_ptr)) throw std::runtime_error(std::string(what) + ": undefined tensor");
+  if (PyObject* cuda = PyObject_GetAttr(t.ptr(), n.is_cuda)) {
+    const bool on_device = py::reinterpret_steal<py::object>(cuda).cast<bool>();
+    if (!on_device)
+      throw std::runtime_error(std::string(what) + ": must be CUDA tensor. got: device=cpu dtype=" + std::string(py::str(t.attr("dtype"))));
+  } else {
+    PyErr_Clear();
+  }
+  const py::tuple shape = as_tuple(attr(t, n.shape));
   const int rank = static_cast<int>(shape.size());
   if (rank > kMaxRank)
     throw std::runtime_error(std::string(what) + ": rank out of range. got rank=" + std::to_string(rank) + " (kMaxRank=" +
                              std::to_string(kMaxRank) + ")");
-  const py::tuple stride = py::tuple(t.attr("stride")());
+  const py::tuple stride = as_tuple(call(t, n.stride));
   d = aicf_tensor_desc{};
-  d.data = reinterpret_cast<void*>(t.attr("data_ptr")().cast<uintptr_t>());
-  d.dtype = static_cast<uint8_t>(dtype_code(t.attr("dtype")));
+  d.data = reinterpret_cast<void*>(call(t, n.data_ptr).cast<uintptr_t>());
+  d.dtype = static_cast<uint8_t>(dtype_code(attr(t, n.dtype)));
   d.rank = rank;
+  if (static_cast<int>(stride.size()) < rank) throw std::runtime_error(std::string(what) + ": fewer strides than extents");
   for (int i = 0; i < rank; ++i) {
-    d.shape[i] = shape[i].cast<int64_t>();
-    d.stride[i] = stride[i].cast<int64_t>();
+    d.shape[i] = as_int(PyTuple_GET_ITEM(shape.ptr(), i));
+    d.stride[i] = as_int(PyTuple_GET_ITEM(stride.ptr(), i));
   }
-  d.contiguous = t.attr("is_contiguous")().cast<bool>() ? 1 : 0;
+  d.contiguous = call(t, n.is_contiguous).cast<bool>() ? 1 : 0;
   d.alignment = 0;  // unknown, as the reference's binding passes it (:122)
   d.device = 0;
 }
