@@ -3,8 +3,8 @@
 The op/attr vocabulary is the reference's (python/aicf_fw/core_v2/lower.py:24-147: Linear ->
 gemm{transB} + bias, LinearBwd -> gemm(dY,W), gemm(dY^T,X), reduce_sum(dY){axis 0}; Stage C fuses
 gemm + bias_add + relu into gemm_epilogue, rewrites/stageC_fuse_epilogue.py:22-74), extended with the
-ops this backend adds: softmax_ce as the loss, the fused Adam that reads the device step counter, bf16
-working copies of fp32 master weights, and all_reduce for data parallelism.
+ops this backend adds: softmax_ce or distill_ce as the loss, block-scaled 8-bit products (linear='fp8'), the fused Adam
+that reads the device step counter, bf16 working copies of fp32 master weights, and all_reduce for data parallelism.
 
 Differences from what the reference's lowering would emit, all of them removing work:
   * the activation saved for relu_bwd is the gemm_epilogue output itself (no copy_saved op),
@@ -24,7 +24,9 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
                          lr: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
                          weight_decay: float = 0.0, data_parallel=False, with_argmax: bool = False,
                          input_f32: bool = True, fuse_relu_bwd: bool = True,
-                         fp32_gemm: str = "exact", fuse_adam: bool = True) -> Tuple[List[ValueSpec], List[Dict[str, Any]]]:
+                         fp32_gemm: str = "exact", fuse_adam: bool = True,
+                         linear: str = "compute", fp8_grad: str = "f8e4m3",
+                         loss: str = "ce", teacher_top: int = 0, temperature: float = 1.0, alpha: float = 0.0) -> Tuple[List[ValueSpec], List[Dict[str, Any]]]:
     """dims = [in, hidden..., out]. Every Linear but the last is followed by ReLU.
 
     compute_dtype 'f32': GEMMs run on fp32 parameters directly.
@@ -40,6 +42,17 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
     fuse_adam: the whole optimizer step is one `adam_step` op over all parameter tensors (kernel
     adam_step_f32_multi_v1) instead of one op per tensor; the arithmetic per element is the same.
 
+    linear: 'compute' multiplies in compute_dtype; 'fp8' (compute_dtype 'bf16' / 'f16') multiplies block-scaled 8-bit
+    matrices. Every weight is quantised per 128 x 128 tile from its fp32 master once per step; activations and their
+    gradients are quantised along the rows and along the columns from one read, because the forward product and the
+    input gradient sum over the columns and the weight gradient over the rows. Activations between the layers, biases,
+    gradients of the parameters and the optimizer are what they are otherwise; there are no 16-bit weight copies.
+    fp8_grad is the format of the activation gradients ('f8e4m3', or 'f8e5m2' for more range and a mantissa bit less).
+
+    loss: 'ce' - softmax cross-entropy of `labels`; 'distill' - distillation from a teacher's top logits: the inputs
+    'teacher.ids' (batch, teacher_top) i32 and 'teacher.logits' (batch, teacher_top) f32 take the place of 'labels', at
+    the given temperature; alpha > 0 mixes in that share of the labels' cross-entropy (and keeps 'labels').
+
     data_parallel: False - single device; True / "nccl" - an all_reduce op per gradient tensor, then the
     ordinary fused Adam; "fused" - one dp_adam_step op per parameter that exchanges the gradient over peer
     memory, updates the owning rank's shard and broadcasts the new weights (master weights and moments of
@@ -51,6 +64,22 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
     fused_dp = dp_mode == "fused"
     cd = compute_dtype
     mixed = cd != "f32"
+    if linear not in ("compute", "fp8"):
+        raise ValueError(f"linear must be 'compute' or 'fp8', got {linear!r}")
+    fp8 = linear == "fp8"
+    if fp8 and not mixed:
+        raise ValueError("linear='fp8' needs 16-bit activations: compute_dtype 'bf16' or 'f16'")
+    if fp8 and fused_dp:
+        raise ValueError("linear='fp8' keeps no 16-bit weight copies, which data_parallel='fused' exchanges; use 'nccl'")
+    if fp8_grad not in ("f8e4m3", "f8e5m2"):
+        raise ValueError(f"fp8_grad must be 'f8e4m3' or 'f8e5m2', got {fp8_grad!r}")
+    if loss not in ("ce", "distill"):
+        raise ValueError(f"loss must be 'ce' or 'distill', got {loss!r}")
+    distill = loss == "distill"
+    if distill and not 1 <= teacher_top <= 1024:
+        raise ValueError(f"loss='distill' needs 1 <= teacher_top <= 1024, got {teacher_top}")
+    if distill and with_argmax:
+        raise ValueError("loss='distill' has no arg-max output")
     gb = int(global_batch or batch)
     vals: List[ValueSpec] = []
     ops: List[Dict[str, Any]] = []
@@ -85,14 +114,34 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
         fused_kid = "gemm_relu_bwd_f32_3xtf32_v0"
     ce_kid = {"f32": "softmax_ce_f32_i32_v0", "bf16": "softmax_ce_bf16_i32_v0", "f16": "softmax_ce_f16_i32_v0"}[cd]
 
+    def blocks(n):
+        return (n + 127) // 128
+
+    def quantise(src, name, shape, forms, fmt):
+        """One quant_fp8 op; returns {form: (values, scales)}."""
+        scale_shape = {"rows": (shape[0], blocks(shape[1])), "cols": (blocks(shape[0]), shape[1]),
+                       "tiles": (blocks(shape[0]), blocks(shape[1]))}
+        made = {f: (val(f"{name}.q_{f}", shape, fmt), val(f"{name}.s_{f}", scale_shape[f], "f32")) for f in forms}
+        op("quant_fp8", [src], [v for f in forms for v in made[f]], None, "quant_fp8_block128_v0")
+        return made
+
+    def fp8_kid(kind, out):
+        return f"{kind}_fp8_block128_out_{out}_v0"
+
     # ---- inputs -------------------------------------------------------------------------------
-    if mixed and input_f32:
+    if fp8 and input_f32:
+        x = val("x", (batch, dims[0]), "f32", ROLE_INPUT)  # quantised as it comes
+    elif mixed and input_f32:
         x_in = val("x", (batch, dims[0]), "f32", ROLE_INPUT)
         x = val("x.lp", (batch, dims[0]), cd)
         op("cast", [x_in], [x], kid="cast_v0")
     else:
         x = val("x", (batch, dims[0]), cd, ROLE_INPUT)
-    labels = val("labels", (batch,), "i32", ROLE_INPUT)
+    if distill:
+        teacher_ids = val("teacher.ids", (batch, teacher_top), "i32", ROLE_INPUT)
+        teacher_logits = val("teacher.logits", (batch, teacher_top), "f32", ROLE_INPUT)
+    if not distill or alpha > 0.0:
+        labels = val("labels", (batch,), "i32", ROLE_INPUT)
 
     # ---- parameters and optimizer state ---------------------------------------------------------
     W, b, Wlp, mW, vW, mb, vb = [], [], [], [], [], [], []
@@ -102,7 +151,7 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
         # copy of a matrix (or the matrix itself in fp32 mode) and the bias
         W.append(val(f"{li}.W", (dims[i + 1], dims[i]), "f32", ROLE_PARAM, peer=fused_dp and not mixed))
         b.append(val(f"{li}.b", (dims[i + 1],), "f32", ROLE_PARAM, peer=fused_dp))
-        Wlp.append(val(f"{li}.W.lp", (dims[i + 1], dims[i]), cd, ROLE_STATIC, persistent=True, peer=fused_dp) if mixed else W[-1])
+        Wlp.append(val(f"{li}.W.lp", (dims[i + 1], dims[i]), cd, ROLE_STATIC, persistent=True, peer=fused_dp) if mixed and not fp8 else W[-1])
         mW.append(val(f"opt.m.{li}.W", (dims[i + 1], dims[i]), "f32", persistent=True))
         vW.append(val(f"opt.v.{li}.W", (dims[i + 1], dims[i]), "f32", persistent=True))
         mb.append(val(f"opt.m.{li}.b", (dims[i + 1],), "f32", persistent=True))
@@ -117,10 +166,18 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
 
     # ---- forward ---------------------------------------------------------------------------------
     acts = [x]
+    qw, qa = [], []  # fp8: each layer's weight in tiles; its input along rows and columns
     for i in range(L):
         last = i == L - 1
         name = "logits" if last else f"relu{i}_out"
         h = val(name, (batch, dims[i + 1]), cd, persistent=last)
+        if fp8:
+            qw.append(quantise(W[i], f"{2 * i}.W", (dims[i + 1], dims[i]), ["tiles"], "f8e4m3")["tiles"])
+            qa.append(quantise(acts[-1], "x" if i == 0 else f"relu{i - 1}_out", (batch, dims[i]), ["rows", "cols"], "f8e4m3"))
+            op("gemm_epilogue", [qa[i]["rows"][0], qw[i][0], b[i], qa[i]["rows"][1], qw[i][1]], [h],
+               {"transB": True, "epilogue": "bias" if last else "bias_relu"}, fp8_kid("gemm_bias_relu", cd))
+            acts.append(h)
+            continue
         op("gemm_epilogue", [acts[-1], Wlp[i], b[i]], [h],
            {"transB": True, "epilogue": "bias" if last else "bias_relu"}, epi_kid)
         acts.append(h)
@@ -129,12 +186,16 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
     # ---- loss ------------------------------------------------------------------------------------
     dlogits = val("d_logits", (batch, dims[-1]), cd)
     loss_row = val("loss_row", (batch,), "f32")
-    loss = val("loss", (1,), "f32", persistent=True)
+    loss_mean = val("loss", (1,), "f32", persistent=True)
     ce_out = [dlogits, loss_row]
     if with_argmax:
         ce_out.append(val("argmax", (batch,), "i32", persistent=True))
-    op("softmax_ce", [logits, labels], ce_out, {"scale": 1.0 / gb}, ce_kid)
-    op("reduce_mean", [loss_row], [loss], None, "reduce_mean_lastaxis_f32_v0")
+    if distill:
+        op("distill_ce", [logits, teacher_ids, teacher_logits] + ([labels] if alpha > 0.0 else []), ce_out,
+           {"scale": 1.0 / gb, "temperature": temperature, "alpha": alpha}, f"distill_ce_{cd}_v0")
+    else:
+        op("softmax_ce", [logits, labels], ce_out, {"scale": 1.0 / gb}, ce_kid)
+    op("reduce_mean", [loss_row], [loss_mean], None, "reduce_mean_lastaxis_f32_v0")
 
     # ---- backward ----------------------------------------------------------------------------------
     dW, db = [None] * L, [None] * L
@@ -143,14 +204,25 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
         li = 2 * i
         dW[i] = val(f"d_{li}.W", (dims[i + 1], dims[i]), "f32", peer=fused_dp)
         db[i] = val(f"d_{li}.b", (dims[i + 1],), "f32", peer=fused_dp)
-        op("gemm", [dY, acts[i]], [dW[i]], {"transA": True, "transB": False}, gemm_f32out_kid)
+        if fp8:
+            qd = quantise(dY, f"d_{'logits' if i == L - 1 else f'relu{i}_out'}", (batch, dims[i + 1]), ["rows", "cols"] if i > 0 else ["cols"], fp8_grad)
+            op("gemm", [qd["cols"][0], qa[i]["cols"][0], qd["cols"][1], qa[i]["cols"][1]], [dW[i]],
+               {"transA": True, "transB": False}, fp8_kid("gemm", "f32"))
+        else:
+            op("gemm", [dY, acts[i]], [dW[i]], {"transA": True, "transB": False}, gemm_f32out_kid)
         op("reduce_sum", [dY], [db[i]], {"axis": 0, "keepdim": False}, colsum_kid)
         if dp_mode == "nccl":
             op("all_reduce", [dW[i]], [dW[i]], {"bucket": 2 * i}, "all_reduce_nccl_f32_v0")
             op("all_reduce", [db[i]], [db[i]], {"bucket": 2 * i + 1}, "all_reduce_nccl_f32_v0")
         if i > 0:
             dX = val(f"d_relu{i - 1}_out", (batch, dims[i]), cd)
-            if fuse_relu_bwd:
+            if fp8 and fuse_relu_bwd:
+                op("gemm_relu_bwd", [qd["rows"][0], qw[i][0], acts[i], qd["rows"][1], qw[i][1]], [dX],
+                   {"transA": False, "transB": False}, fp8_kid("gemm_relu_bwd", cd))
+            elif fp8:
+                op("gemm", [qd["rows"][0], qw[i][0], qd["rows"][1], qw[i][1]], [dX], {"transA": False, "transB": False}, fp8_kid("gemm", cd))
+                op("relu_bwd", [dX, acts[i]], [dX], None, relu_bwd_kid)
+            elif fuse_relu_bwd:
                 op("gemm_relu_bwd", [dY, Wlp[i], acts[i]], [dX], {"transA": False, "transB": False}, fused_kid)
             else:
                 op("gemm", [dY, Wlp[i]], [dX], {"transA": False, "transB": False}, gemm_kid)
@@ -176,7 +248,7 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
         # one launch for all 2L parameter tensors: inputs [P,G,M,V] per tensor then the step counter; outputs
         # [P,M,V(,working copy)] per tensor
         ins, outs, mask = [], [], 0
-        for t, (P, G, Mo, Vo, lp) in enumerate([(W[i], dW[i], mW[i], vW[i], Wlp[i] if mixed else None) for i in range(L)] +
+        for t, (P, G, Mo, Vo, lp) in enumerate([(W[i], dW[i], mW[i], vW[i], Wlp[i] if mixed and not fp8 else None) for i in range(L)] +
                                                [(b[i], db[i], mb[i], vb[i], None) for i in range(L)]):
             ins += [P, G, Mo, Vo]
             outs += [P, Mo, Vo] + ([lp] if lp is not None else [])
@@ -184,7 +256,7 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
         op("adam_step", ins + [step], outs, dict(hyper, count=2 * L, lp_mask=mask), "adam_step_f32_multi_v1")
         return vals, ops
     for i in range(L):
-        outs = [W[i], mW[i], vW[i]] + ([Wlp[i]] if mixed else [])
+        outs = [W[i], mW[i], vW[i]] + ([Wlp[i]] if mixed and not fp8 else [])
         op("adam_step", [W[i], dW[i], mW[i], vW[i], step], outs, hyper, "adam_step_f32_fused_v1")
         op("adam_step", [b[i], db[i], mb[i], vb[i], step], [b[i], mb[i], vb[i]], hyper, "adam_step_f32_fused_v1")
     return vals, ops
