@@ -132,7 +132,7 @@ template <int kCg, int kTn, bool kVecB> struct Cfg {
   static constexpr int kRegsLaunch = 168, kRegsRoles = 56, kRegsEpi = 224;
   static_assert(128 * kRegsRoles + 32 * kEpiWarps * kRegsEpi <= kThreads * kRegsLaunch, "the warpgroups' shares come out of the block's registers");
   static constexpr int kCols = kTn / (kEpiWarps / 4);       // columns per epilogue warp
-    // columns per TMEM load: two sets of 32 next to 128 sums spill (599 against 480 us at 8192^3); next to 64 they are faster
+  // columns per TMEM load: two sets of 32 next to 128 sums spill (599 against 480 us at 8192^3); next to 64 they are faster
   // (609 against 637 us), unless the columns' factors want registers, too (937 against 811 us for the weight gradient)
   static constexpr int kCh = kCols == 64 && !kVecB ? 32 : 16;
   // staged scales: two groups of kScaleGroup k blocks, each the rows' and then the columns' factors
@@ -240,6 +240,10 @@ __device__ __forceinline__ float4 lds4(uint32_t a) {
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
   return v;
 }
+// Four bytes from global to shared memory, or zeros.
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
 // The product of two scales, held inside fp32's range: a block of zeros stays zero whatever its scales. A NaN stays one.
 __device__ __forceinline__ float clamp_finite(float v) {
   float r;
@@ -264,7 +268,15 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t* w) {
 }
 
 // 32 consecutive columns of one row of C: bias and ReLU, or the ReLU-backward mask; convert; store.
-__device__ __forceinline__ void finish32(const Fp8Params& p, int row, int col0, float (&v)[32]) {
+// `ahead`: the 16-bit mask of these columns, loaded before the columns before them were finished.
+__device__ __forceinline__ void load_mask32(const Fp8Params& p, int row, int col0, uint4 (&ahead)[4]) {
+  if (p.mask && p.mask_vec && p.c_dtype != static_cast<int>(DType::kF32) && row < p.M && col0 + 32 <= p.N) {
+    const uint4* ms = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.mask) + static_cast<int64_t>(row) * p.mask_ld + col0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) ahead[q] = __ldcs(ms + q);
+  }
+}
+__device__ __forceinline__ void finish32(const Fp8Params& p, int row, int col0, float (&v)[32], const uint4 (&ahead)[4]) {
   if (p.bias_vec && col0 + 32 <= p.N) {  // the same address in every lane
     const float4* b = reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + col0);
 #pragma unroll
@@ -285,13 +297,10 @@ __device__ __forceinline__ void finish32(const Fp8Params& p, int row, int col0, 
   const bool whole = col0 + 32 <= p.N;
   const bool f32 = p.c_dtype == static_cast<int>(DType::kF32), bf16 = p.c_dtype == static_cast<int>(DType::kBF16);
   if (p.mask) {
-    const int64_t moff = static_cast<int64_t>(row) * p.mask_ld + col0;
     if (whole && p.mask_vec && !f32) {
-      const uint4* ms = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.mask) + moff);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const uint4 y = __ldcs(ms + q);
-        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+        const uint32_t w[4] = {ahead[q].x, ahead[q].y, ahead[q].z, ahead[q].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float lo, hi;
@@ -306,6 +315,7 @@ __device__ __forceinline__ void finish32(const Fp8Params& p, int row, int col0, 
         }
       }
     } else {
+      const int64_t moff = static_cast<int64_t>(row) * p.mask_ld + col0;
 #pragma unroll
       for (int j = 0; j < 32; ++j)
         if (col0 + j < p.N && !(load_as_f32(p.mask, moff + j, p.c_dtype) > 0.0f)) v[j] = 0.0f;
@@ -375,7 +385,6 @@ __global__ void __launch_bounds__(Cfg<kCg, kTn, kVecB>::kThreads, 1)
   const uint32_t bar_full = base + kRingBytes, bar_empty = bar_full + 8 * F::kStages,
                  bar_acc_empty = bar_empty + 8 * F::kStages, bar_sc_full = bar_acc_empty + 8 * F::kBufs, bar_sc_empty = bar_sc_full + 16;
   uint8_t* misc = base_ptr + kRingBytes + 16 * F::kStages + 8 * F::kBufs + 32;
-  float* scales = reinterpret_cast<float*>(base_ptr + kRingBytes + 256);
   const uint32_t scales_a = base + kRingBytes + 256;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
@@ -401,7 +410,7 @@ __global__ void __launch_bounds__(Cfg<kCg, kTn, kVecB>::kThreads, 1)
     }
     for (int b = 0; b < F::kBufs; ++b) mbar_init(bar_acc_empty + 8 * b, kCg * F::kEpiWarps);
     for (int g = 0; g < 2; ++g) {
-      mbar_init(bar_sc_full + 8 * g, 2);           // the two scale warps
+      mbar_init(bar_sc_full + 8 * g, 64);          // the two scale warps' threads, when their copies have landed
       mbar_init(bar_sc_empty + 8 * g, F::kEpiWarps);
     }
     *abort_flag = 0;
@@ -505,34 +514,44 @@ __global__ void __launch_bounds__(Cfg<kCg, kTn, kVecB>::kThreads, 1)
       int tm, tn;
       tile_of(item, tiles_m, tiles_n, max(kGroupM / kCg, 1), &tm, &tn);
       const int m0 = (tm * kCg + (kCg == 2 ? static_cast<int>(rank) : 0)) * kTileM, n0 = tn * kTn;
+      if (p.mask) {
+        // the tile of the mask, on its way to L2 while the tile is multiplied: the input gradient of [65536,1000] x
+        // [1000,8192] takes 710 us without a mask, 2250 with one read from HBM where it is used, 1310 so. (Turned into bits
+        // here, it was 1250..3000 us and slowed the other products, in the epilogue before the tile 1700.)
+        const int bytes = p.c_dtype == static_cast<int>(DType::kF32) ? 4 : 2;
+        for (int i = t; i < kTileM * (kTn * bytes / 128); i += 64) {
+          const int row = m0 + i % kTileM, col = n0 + i / kTileM * (128 / bytes);
+          if (row < p.M && col < p.N)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(p.mask) + (static_cast<int64_t>(row) * p.mask_ld + col) * bytes));
+        }
+      }
       for (int kb0 = kb_lo; kb0 < kb_hi; kb0 += kScaleGroup) {
         if (!warp_wait(bar_sc_empty + 8 * g, g_phase ^ 1u, abort_flag, 5)) { alive = false; break; }
-        float* rows_s = scales + g * F::kGroupFloats;
-        float* cols_s = rows_s + kScaleGroup * kTileM;
+        // 4-byte asynchronous copies: nothing waits for one, and what lies outside the matrix becomes 0. (With loads through
+        // registers, eight at a time, staging was what the weight gradient waited for.)
+        const uint32_t rows_a = scales_a + 4 * g * F::kGroupFloats, cols_a = rows_a + 4 * kScaleGroup * kTileM;
         const int n = min(kScaleGroup, kb_hi - kb0);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int row = m0 + t + 64 * h;
-          const float* src = p.sa.data + (row / p.sa.per) * p.sa.smn + kb0 * p.sa.sk;
-#pragma unroll
-          for (int q = 0; q < kScaleGroup; ++q)
-            rows_s[q * kTileM + t + 64 * h] = row < p.M && q < n ? __ldg(src + q * p.sa.sk) : 0.0f;
+          const bool in = row < p.M;
+          const float* src = p.sa.data + (in ? (row / p.sa.per) * p.sa.smn + kb0 * p.sa.sk : 0);
+          for (int q = 0; q < n; ++q, src += in ? p.sa.sk : 0) copy4(rows_a + 4 * (q * kTileM + t + 64 * h), src, in);
         }
         if constexpr (kVecB) {
-#pragma unroll
+#pragma unroll 1
           for (int h = 0; h < kTn / 64; ++h) {
             const int col = n0 + t + 64 * h;
-            const float* src = p.sb.data + col * p.sb.smn + kb0 * p.sb.sk;
-#pragma unroll
-            for (int q = 0; q < kScaleGroup; ++q)
-              cols_s[q * kTn + t + 64 * h] = col < p.N && q < n ? __ldg(src + q * p.sb.sk) : 0.0f;
+            const bool in = col < p.N;
+            const float* src = p.sb.data + (in ? col * p.sb.smn + kb0 * p.sb.sk : 0);
+            for (int q = 0; q < n; ++q, src += in ? p.sb.sk : 0) copy4(cols_a + 4 * (q * kTn + t + 64 * h), src, in);
           }
-        } else if (t < 2 * kScaleGroup) {
+        } else if (t < 2 * n) {
           const int q = t >> 1, blk = n0 / kScaleBlk + (t & 1);  // a tile narrower than 128 columns lies in one block
-          cols_s[t] = blk * kScaleBlk < p.N && q < n ? __ldg(p.sb.data + blk * p.sb.smn + (kb0 + q) * p.sb.sk) : 0.0f;
+          const bool in = blk * kScaleBlk < p.N;
+          copy4(cols_a + 4 * t, p.sb.data + (in ? blk * p.sb.smn + (kb0 + q) * p.sb.sk : 0), in);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_sc_full + 8 * g);
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_sc_full + 8 * g) : "memory");
         if (++g == 2) { g = 0; g_phase ^= 1u; }
       }
     }
@@ -549,8 +568,8 @@ __global__ void __launch_bounds__(Cfg<kCg, kTn, kVecB>::kThreads, 1)
     for (int item = first_item; item < items && alive; item += item_step) {
       int tm, tn;
       tile_of(item, tiles_m, tiles_n, max(kGroupM / kCg, 1), &tm, &tn);
-      const int row = (tm * kCg + (kCg == 2 ? static_cast<int>(rank) : 0)) * kTileM + sub * 32 + lane;
-      const int col0 = tn * kTn + half * kCols;
+      int row = (tm * kCg + (kCg == 2 ? static_cast<int>(rank) : 0)) * kTileM + sub * 32 + lane;
+      int col0 = tn * kTn + half * kCols;
       const bool idle = row - lane >= p.M || col0 >= p.N;  // nothing of this warp's part is stored: it only keeps pace
       uint64_t acc[kCols / 2];
 #pragma unroll
@@ -653,6 +672,12 @@ __global__ void __launch_bounds__(Cfg<kCg, kTn, kVecB>::kThreads, 1)
         if (++g == 2) { g = 0; g_phase ^= 1u; }
       }
       if (!alive) break;
+      // the tile's place again: carried through the loop above it would cost registers that the sums need
+      int again = item;
+      asm volatile("" : "+r"(again));
+      tile_of(again, tiles_m, tiles_n, max(kGroupM / kCg, 1), &tm, &tn);
+      row = (tm * kCg + (kCg == 2 ? static_cast<int>(rank) : 0)) * kTileM + sub * 32 + lane;
+      col0 = tn * kTn + half * kCols;
       if (splits > 1) {
         // this CTA's part of the sum, parked where the ring was: its last MMA has read it, and no load is in flight
         float* park = reinterpret_cast<float*>(base_ptr) + (sub * 32 + lane) * (kTn + 4) + half * kCols;
@@ -663,8 +688,11 @@ __global__ void __launch_bounds__(Cfg<kCg, kTn, kVecB>::kThreads, 1)
         }
         break;  // a split cluster has one item
       }
+      uint4 ahead[2][4];
+      load_mask32(p, row, col0, ahead[0]);
 #pragma unroll
       for (int c = 0; c < kCols / 32; ++c) {
+        if (c + 1 < kCols / 32) load_mask32(p, row, col0 + 32 * (c + 1), ahead[(c + 1) & 1]);
         if (col0 + 32 * c < p.N) {
           float v[32];
 #pragma unroll
@@ -672,7 +700,7 @@ __global__ void __launch_bounds__(Cfg<kCg, kTn, kVecB>::kThreads, 1)
             const float2 a = unpack2(acc[16 * c + j]);
             v[2 * j] = a.x, v[2 * j + 1] = a.y;
           }
-          finish32(p, row, col0 + 32 * c, v);
+          finish32(p, row, col0 + 32 * c, v, ahead[c & 1]);
         }
       }
       __syncwarp();
@@ -712,6 +740,7 @@ __global__ void __launch_bounds__(Cfg<kCg, kTn, kVecB>::kThreads, 1)
       cluster_sync_all();  // nobody leaves while a peer may still be reading its shared memory
     }
   }
+  if (warp == 2 || warp == 3) asm volatile("cp.async.wait_all;" ::: "memory");
   if (*abort_flag) {
     // error path only: give loads that may still be in flight time to land before shared memory is released
     for (int i = 0; i < 64; ++i) __nanosleep(16384);
@@ -800,10 +829,11 @@ struct Choice {
 };
 // Tile shape by a cost model: rounds of tiles over the SMs (or SM pairs), each round the time of a tile's k blocks and of
 // storing it. The times are those of one round, measured at K = 8192 and K = 1000 (microseconds per k block / per tile stored):
-//   256 x 256, CTA pair   0.54, or 0.78 with a factor per column of B   2.1
-//   128 x 256             0.56 / 0.81                                   2.0
-//   128 x 128             0.34 / 0.45                                   1.0
-//   128 x 64              0.27 / 0.30                                   0.6
+//                           k block, with a factor per column of B   stored, with a mask
+//   256 x 256, CTA pair     0.54       0.72                            2.1     9.2
+//   128 x 256               0.56       0.74                            2.0     7.3
+//   128 x 128               0.34       0.45                            1.0     4.0
+//   128 x 64                0.27       0.30                            0.6     2.2
 // The narrow tiles may share K among the CTAs of a cluster (which costs about 3 us for the exchange): that is for few rows,
 // where one round of unsplit tiles leaves each CTA a long serial walk along K (M = 1, 8192 x 8192: 33.7 us unsplit on 128 x 64
 // tiles, 28.9 as two halves of 128 x 128).
@@ -813,8 +843,9 @@ Choice choose(const Fp8Problem& q, bool b_n_major) {
   const int64_t sms = sm_count(), kb = blocks_of(g.K);
   const bool vec = q.sb.per == 1;
   struct Shape { int cg, tn; double block, store; };
-  const Shape shapes[4] = {{2, 256, vec ? 0.78 : 0.54, 2.1}, {1, 256, vec ? 0.81 : 0.56, 2.0}, {1, 128, vec ? 0.45 : 0.34, 1.0},
-                           {1, 64, vec ? 0.30 : 0.27, 0.6}};
+  const bool mask = g.mask != nullptr;
+  const Shape shapes[4] = {{2, 256, vec ? 0.72 : 0.54, mask ? 9.2 : 2.1}, {1, 256, vec ? 0.74 : 0.56, mask ? 7.3 : 2.0},
+                           {1, 128, vec ? 0.45 : 0.34, mask ? 4.0 : 1.0}, {1, 64, vec ? 0.30 : 0.27, mask ? 2.2 : 0.6}};
   Choice best;
   double best_cost = 1e300;
   for (const Shape& s : shapes) {
