@@ -98,3 +98,23 @@ def test_captured_and_replayed(gpu):
     _C.graph_reset()
     wq, ws = oracle.quant_fp8(2 * x, "rows", "f8e4m3")
     assert np.array_equal(q.float_numpy(), wq) and np.array_equal(s.float_numpy(), ws)
+
+
+@pytest.mark.parametrize("fmt", ["f8e4m3", "f8e5m2"])
+@pytest.mark.parametrize("power", [-100, -60, 0, 60, 127])
+def test_quotients_next_to_a_tie_round_to_the_right_side(gpu, fmt, power):
+    """Values within half an fp32 step of the midpoint between two values of the format: the fp32 quotient often is the
+    midpoint itself, and only the exact one tells the side."""
+    rng = np.random.default_rng(power + 200)
+    M, N = 256, 1024
+    amax = (np.float64(2.0) ** power * rng.uniform(1.0, 1.99, (M, N // 128))).astype(np.float32).astype(np.float64)
+    bits = 3 if fmt == "f8e4m3" else 2
+    top = 8 if fmt == "f8e4m3" else 15
+    mid = (2 ** bits + rng.integers(0, 2 ** bits, (M, N)) + 0.5) * 2.0 ** (rng.integers(-6, top, (M, N)) - bits)
+    x = (mid * np.repeat(amax, 128, axis=1) / (448.0 if fmt == "f8e4m3" else 57344.0)).astype(np.float32)
+    x *= rng.choice(np.float32([-1, 1]), (M, N))
+    x[:, ::128] = amax
+    for form in ("rows", "cols", "tiles"):
+        xs, (q, s) = quantise(x, "f32", [form], [fmt])
+        wq, ws = oracle.quant_fp8(xs, form, fmt)
+        assert np.array_equal(s.float_numpy(), ws) and np.array_equal(q.float_numpy(), wq), form
