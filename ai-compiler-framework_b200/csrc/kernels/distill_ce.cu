@@ -41,8 +41,9 @@ struct DistillParams {
   int64_t B, C;
   int K;
   float scale, temperature, alpha;
-  // from these: log2(e) / T; the weights of both terms in the gradient, scale (1 - alpha) T and scale alpha; (1 - alpha) T^2
-  float cT, grad_soft, grad_hard, loss_soft;
+  // from these: 1 / T and log2(e) / T; the weights of both terms in the gradient, scale (1 - alpha) T and scale alpha;
+  // (1 - alpha) T^2
+  float invT, cT, grad_soft, grad_hard, loss_soft;
 };
 
 __device__ __forceinline__ float teacher_at(const DistillParams& p, int64_t i) {
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(256) distill_multipass_kernel(const DistillPar
 // ------------------------------------------------------------------ one read, one write
 // Exponentials are taken in powers of two: with c = log2(e) / T and n = max(z) c, rounded to fp32, softmax(z / T) is
 // 2^(z c - n) / S, S the sum of the numerators. z c - n is one fused multiply-add, so n is an exact reference and a logit
-// costs three instructions. The three kinds of row differ in who holds it:
+// costs three instructions. (Rows whose maximum is a mask's lowest value: see far_off.) The three kinds of row differ in who holds it:
 //
 //   distill_warp_kernel    up to 2048 columns: one warp per row, the row in its registers, many short blocks
 //   distill_block_kernel   longer rows: one CTA, or one per slice of the row in a cluster, the slice in shared memory; two or
@@ -176,11 +177,25 @@ enum ExpMode : int {
   kTwoExps = 2,   // any other T
 };
 
+// n is off by up to half a step of its own size, and a logit of -1e30, the lowest value of its type above all, makes it too
+// large for that (or infinite) although the differences inside the row are small. Where |n| >= 2^31 (squared exponentials:
+// 2^29), neighbouring fp32 values near the maximum are 128 (32) apart in the exponent, so every logit below it weighs nothing
+// (2^-32 at most) and every logit equal to it 1: any power of two of at least c says that without a rounding. 1 is one where
+// the maximum is 2^40 or more, and the power above c stays in range otherwise (T is held to [2^-60, 2^60]).
+template <int kMode>
+__device__ __forceinline__ bool far_off(float n) { return !(fabsf(n) < (kMode == kSquares ? 0x1p29f : 0x1p31f)); }
+template <int kMode>
+__device__ __forceinline__ float factor_of(float ref, float c) {
+  if (!far_off<kMode>(__fmul_rn(ref, c))) return c;
+  return fabsf(ref) >= 0x1p40f ? 1.0f : __uint_as_float((__float_as_uint(c) & 0x7F800000u) + 0x00800000u);
+}
+
 // What a row's softmaxes come down to, in every thread.
 struct RowStats {
-  float n, S, S1;   // reference and sum at temperature T, sum at 1 (its reference: T n where squared, else n1)
-  float n1;
-  float nt, St;     // teacher
+  float ref;        // the maximum the exponentials refer to
+  float c, n, S;    // factor, reference and sum at temperature T
+  float c1, n1, S1; // at 1 (where squared, the sum's reference is T n)
+  float ct, nt, St; // teacher
   bool some, known; // has a target, has a label
   float kT, k1;     // factors of the two numerators in the gradient
 };
@@ -215,33 +230,57 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t v) {
   const float2 u = split(v);
   return pair(ex2(u.x), ex2(u.y));
 }
-// Exponentials of one row. `c` is log2(e) / T for the distillation term, `c1` log2(e) for the label term.
+// Exponentials of one row: log2(e) / T for the distillation term, log2(e) for the label term.
 template <int kMode>
 struct Exps {
-  float cT, c1;
+  float cT;
   int squarings;
-  // reference of the label term's exponentials that goes with reference `ref` (a logit) of the others
-  __device__ __forceinline__ float n1_of(float ref) const { return __fmul_rn(ref, c1); }
-  __device__ __forceinline__ uint64_t numerators1(uint64_t v, uint64_t e, float n1) const {
+  __device__ __forceinline__ void refer(float m, RowStats& r) const {
+    r.ref = m == -INFINITY ? 0.0f : m;
+    r.c = factor_of<kMode>(r.ref, cT);
+    r.n = __fmul_rn(r.ref, r.c);
+    if constexpr (kMode == kOneExp) {
+      r.c1 = r.c, r.n1 = r.n;
+    } else {
+      r.c1 = factor_of<kTwoExps>(r.ref, kLog2e);
+      r.n1 = __fmul_rn(r.ref, r.c1);
+    }
+  }
+  // what a sum with maximum `a` counts for in one with maximum m
+  __device__ __forceinline__ float weight(float a, float m, float c) const {
+    const float na = __fmul_rn(a, c), nm = __fmul_rn(m, c);
+    if (a == m) return 1.0f;
+    if (far_off<kMode>(nm)) return 0.0f;
+    return ex2(far_off<kMode>(na) ? fmaf(a, c, -nm) : na - nm);
+  }
+  // the same for the sum at 1: squared sums refer to T n, so their weights are the others' squared
+  __device__ __forceinline__ float weight1(float a, float m) const {
+    if constexpr (kMode == kSquares) {
+      const float w = weight(a, m, cT), w2 = w * w;
+      return squarings == 2 ? w2 * w2 : w2;
+    }
+    return weight(a, m, kLog2e);
+  }
+  __device__ __forceinline__ uint64_t numerators1(uint64_t v, uint64_t e, const RowStats& r) const {
     if constexpr (kMode == kSquares) {
       const uint64_t e2 = mul2(e, e);
       return squarings == 2 ? mul2(e2, e2) : e2;
     }
-    if constexpr (kMode == kTwoExps) return ex2_pair(fma2(v, pair(c1, c1), pair(-n1, -n1)));
+    if constexpr (kMode == kTwoExps) return ex2_pair(fma2(v, pair(r.c1, r.c1), pair(-r.n1, -r.n1)));
     return e;
   }
-  __device__ __forceinline__ void add(uint64_t v, float n, float n1, uint64_t& s, uint64_t& s1) const {
-    const uint64_t e = ex2_pair(fma2(v, pair(cT, cT), pair(-n, -n)));
+  __device__ __forceinline__ void add(uint64_t v, const RowStats& r, uint64_t& s, uint64_t& s1) const {
+    const uint64_t e = ex2_pair(fma2(v, pair(r.c, r.c), pair(-r.n, -r.n)));
     s = add2(s, e);
-    if constexpr (kMode != kOneExp) s1 = add2(s1, numerators1(v, e, n1));
+    if constexpr (kMode != kOneExp) s1 = add2(s1, numerators1(v, e, r));
   }
   __device__ __forceinline__ uint64_t grad(uint64_t v, const RowStats& r) const {
-    const uint64_t e = ex2_pair(fma2(v, pair(cT, cT), pair(-r.n, -r.n)));
+    const uint64_t e = ex2_pair(fma2(v, pair(r.c, r.c), pair(-r.n, -r.n)));
     if constexpr (kMode == kOneExp) return mul2(e, pair(r.kT, r.kT));  // kT holds both factors
     if constexpr (kMode == kSquares) {
       if (squarings == 1) return mul2(e, fma2(e, pair(r.k1, r.k1), pair(r.kT, r.kT)));
     }
-    return fma2(numerators1(v, e, r.n1), pair(r.k1, r.k1), mul2(e, pair(r.kT, r.kT)));
+    return fma2(numerators1(v, e, r), pair(r.k1, r.k1), mul2(e, pair(r.kT, r.kT)));
   }
   __device__ __forceinline__ float grad1(float v, const RowStats& r) const { return split(grad(pair(v, v), r)).x; }
 };
@@ -285,14 +324,27 @@ __device__ __forceinline__ void finish_stats(const DistillParams& p, bool known,
   r.k1 = known ? quotient(p.grad_hard, r.S1) : 0.0f;
   if (kMode == kOneExp) r.kT += r.k1;
 }
-// p_k
-__device__ __forceinline__ float target(const DistillParams& p, const RowStats& r, float t) {
-  return r.some ? quotient(ex2(fmaf(t, p.cT, -r.nt)), r.St) : 0.0f;
+// The teacher's reference: its largest logit as it stands, and what follows from it.
+__device__ __forceinline__ void refer_teacher(const DistillParams& p, float mt, RowStats& r) {
+  const float ref = mt == -INFINITY ? 0.0f : mt;
+  r.ct = factor_of<kOneExp>(ref, p.cT);
+  r.nt = __fmul_rn(ref, r.ct);
 }
-// p_k (log2 p_k - log2 q_k) without the sums' logarithms
+__device__ __forceinline__ float teacher_weight(const RowStats& r, float t) { return ex2(fmaf(t, r.ct, -r.nt)); }
+// p_k
+__device__ __forceinline__ float target(const RowStats& r, float t) { return r.some ? quotient(teacher_weight(r, t), r.St) : 0.0f; }
+constexpr float kLn2 = 0.6931471805599453f;
+// log q (at temperature 1 / inv) of a logit, without the sum's logarithm: by the factors of the row's exponentials, or, where
+// these do not hold a difference as large, from the logits themselves
+__device__ __forceinline__ float log_numerator(float zv, float ref, float c, float n, bool far, float inv) {
+  const float l = kLn2 * fmaf(zv, c, -n);
+  return l > -0x1p30f && !far ? l : (zv - ref) * inv;
+}
+// p_k (log p_k - log q_k) without the sums' logarithms
+template <int kMode>
 __device__ __forceinline__ float cross_term(const DistillParams& p, const RowStats& r, float t, float zv) {
-  const float a = fmaf(t, p.cT, -r.nt), pk = target(p, r, t);
-  return pk != 0.0f ? pk * (a - fmaf(zv, p.cT, -r.n)) : 0.0f;
+  const float pk = target(r, t);
+  return pk != 0.0f ? pk * (kLn2 * fmaf(t, r.ct, -r.nt) - log_numerator(zv, r.ref, r.c, r.n, far_off<kMode>(r.n), p.invT)) : 0.0f;
 }
 // The loss is what the sums contribute plus what the list's (`cross`: the sum of cross_term) and the label's logits do.
 __device__ __forceinline__ float loss_of_sums(const DistillParams& p, const RowStats& r) {
@@ -301,10 +353,10 @@ __device__ __forceinline__ float loss_of_sums(const DistillParams& p, const RowS
   if (r.known) loss += p.alpha * logf(r.S1);
   return loss;
 }
-constexpr float kLn2 = 0.6931471805599453f;
-__device__ __forceinline__ float loss_of_list(const DistillParams& p, float cross) { return p.loss_soft * (kLn2 * cross); }
-__device__ __forceinline__ float loss_of_label(const DistillParams& p, const RowStats& r, float z_label, float c1) {
-  return -p.alpha * (kLn2 * fmaf(z_label, c1, -r.n1));
+__device__ __forceinline__ float loss_of_list(const DistillParams& p, float cross) { return p.loss_soft * cross; }
+template <int kMode>
+__device__ __forceinline__ float loss_of_label(const DistillParams& p, const RowStats& r, float z_label) {
+  return -p.alpha * log_numerator(z_label, r.ref, r.c1, r.n1, kMode == kSquares ? far_off<kMode>(r.n) : far_off<kMode>(r.n1), 1.0f);
 }
 __device__ __forceinline__ float max_of(const Pack16<float>& v) { return fmaxf(fmaxf(v.v[0], v.v[1]), fmaxf(v.v[2], v.v[3])); }
 __device__ __forceinline__ float max_of(const Pack16<__nv_bfloat16>& v) {
@@ -346,7 +398,7 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock, kPk * Pack16<T>::kN <= 32 
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + warp;
   if (row >= p.B) return;  // whole warps: nothing below meets another warp
   const bool hard = p.labels != nullptr && p.alpha > 0.0f;
-  const Exps<kMode> x{p.cT, kLog2e, g.squarings};
+  const Exps<kMode> x{p.cT, g.squarings};
   const T* z = static_cast<const T*>(p.z) + row * p.ldz;
   const int C = static_cast<int>(p.C);
   const int head = head_elements(z, p.C);
@@ -382,11 +434,10 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock, kPk * Pack16<T>::kN <= 32 
   bool twice = false;
   bool known;
   {
-    float nt = my_col >= 0 && lane < p.K ? my_t * p.cT : -INFINITY;
+    float mt = my_col >= 0 && lane < p.K ? my_t : -INFINITY;
     if constexpr (kOneEach) {
-      r.nt = warp_max(nt);
-      if (r.nt == -INFINITY) r.nt = 0.0f;
-      r.St = warp_sum(my_col >= 0 && lane < p.K ? ex2(fmaf(my_t, p.cT, -r.nt)) : 0.0f);
+      refer_teacher(p, warp_max(mt), r);
+      r.St = warp_sum(my_col >= 0 && lane < p.K ? teacher_weight(r, my_t) : 0.0f);
       known = __shfl_sync(0xffffffffu, my_col, p.K) >= 0;
     } else {
       for (int i = lane; i < words; i += 32) bits_s[i] = 0u;
@@ -395,15 +446,14 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock, kPk * Pack16<T>::kN <= 32 
         if (k != lane) load_entry(k, &my_col, &my_t, &my_z);
         col_s[k] = my_col, t_s[k] = my_t, z_s[k] = my_z;
         if (my_col < 0) continue;
-        if (k < p.K) nt = fmaxf(nt, my_t * p.cT);
+        if (k < p.K) mt = fmaxf(mt, my_t);
         if (p.dz && (atomicOr(bits_s + (my_col >> 5), 1u << (my_col & 31)) & (1u << (my_col & 31)))) twice = true;
       }
-      r.nt = warp_max(nt);
-      if (r.nt == -INFINITY) r.nt = 0.0f;
+      refer_teacher(p, warp_max(mt), r);
       __syncwarp();
       float st = 0.0f;
       for (int k = lane; k < p.K; k += 32)
-        if (col_s[k] >= 0) st += ex2(fmaf(t_s[k], p.cT, -r.nt));
+        if (col_s[k] >= 0) st += teacher_weight(r, t_s[k]);
       r.St = warp_sum(st);
       known = col_s[p.K] >= 0;
     }
@@ -413,18 +463,16 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock, kPk * Pack16<T>::kN <= 32 
   for (int q = 0; q < kPk; ++q)
     if (lane + 32 * q < pn) m = fmaxf(m, max_of(raw[q]));
   m = warp_max(m);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  r.n = __fmul_rn(ref, p.cT);
-  r.n1 = x.n1_of(ref);
+  x.refer(m, r);
   uint64_t s2 = pair(0.0f, 0.0f), s12 = s2;
-  if (edges > 0) x.add(pair(fe, -INFINITY), r.n, r.n1, s2, s12);  // lanes without an edge element add zeros
+  if (edges > 0) x.add(pair(fe, -INFINITY), r, s2, s12);  // lanes without an edge element add zeros
 #pragma unroll
   for (int q = 0; q < kPk; ++q)
     if (lane + 32 * q < pn) {
       uint64_t v[kN / 2];
       unpack_pairs<T>(raw[q], v);
 #pragma unroll
-      for (int e = 0; e < kN / 2; ++e) x.add(v[e], r.n, r.n1, s2, s12);
+      for (int e = 0; e < kN / 2; ++e) x.add(v[e], r, s2, s12);
     }
   {
     const float2 a = split(s2), b = split(s12);
@@ -435,16 +483,16 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock, kPk * Pack16<T>::kN <= 32 
   float own = 0.0f;
   if (r.some) {
     if constexpr (kOneEach) {
-      own = my_col >= 0 && lane < p.K ? cross_term(p, r, my_t, my_z) : 0.0f;
+      own = my_col >= 0 && lane < p.K ? cross_term<kMode>(p, r, my_t, my_z) : 0.0f;
     } else {
       for (int k = lane; k < p.K; k += 32)
-        if (col_s[k] >= 0) own += cross_term(p, r, t_s[k], z_s[k]);
+        if (col_s[k] >= 0) own += cross_term<kMode>(p, r, t_s[k], z_s[k]);
     }
     own = loss_of_list(p, warp_sum(own));
   }
   if (known) {
-    if constexpr (kOneEach) own += loss_of_label(p, r, __shfl_sync(0xffffffffu, my_z, p.K), x.c1);
-    else own += loss_of_label(p, r, z_s[p.K], x.c1);
+    if constexpr (kOneEach) own += loss_of_label<kMode>(p, r, __shfl_sync(0xffffffffu, my_z, p.K));
+    else own += loss_of_label<kMode>(p, r, z_s[p.K]);
   }
   if (lane == 0) p.loss[row] = loss_of_sums(p, r) + own;
   if (!p.dz) return;
@@ -470,7 +518,7 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock, kPk * Pack16<T>::kN <= 32 
   // The corrections come behind the row: other lanes, the same addresses. Equal columns are corrected once, by their first
   // entry, for the sum of their weights in the list's order.
   if constexpr (kOneEach) {
-    float w = lane == p.K ? p.grad_hard : p.grad_soft * target(p, r, my_t);
+    float w = lane == p.K ? p.grad_hard : p.grad_soft * target(r, my_t);
     bool first = my_col >= 0;
     const uint32_t same = __match_any_sync(0xffffffffu, first ? my_col : -1 - lane);
     if (__any_sync(0xffffffffu, (same & (same - 1)) != 0u)) {
@@ -492,7 +540,7 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock, kPk * Pack16<T>::kN <= 32 
       if (col < 0) continue;
       float w = 0.0f;
       bool first = true;
-      auto weight = [&](int j) { return j == p.K ? p.grad_hard : p.grad_soft * target(p, r, t_s[j]); };
+      auto weight = [&](int j) { return j == p.K ? p.grad_hard : p.grad_soft * target(r, t_s[j]); };
       if (dup) {
         for (int j = 0; j < entries; ++j)
           if (col_s[j] == col) {
@@ -550,7 +598,7 @@ __global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kern
   float* t_s = reinterpret_cast<float*>(col_s + entries);
   float* z_s = t_s + entries;
   __shared__ float red[2][3][kRowThreads / 32];
-  __shared__ float teach[2][3];            // the teacher's reference and sum; whether the row has a label
+  __shared__ float teach[2][4];            // the teacher's factor, reference and sum; whether the row has a label
   __shared__ float peer[2][kMaxRanks][4];  // per CTA of the cluster: maximum, two sums, and its part of the loss
   __shared__ int wait_failed;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -560,7 +608,7 @@ __global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kern
   const int64_t first_row = g.ranks > 1 ? cluster_index() : blockIdx.x, row_step = g.ranks > 1 ? cluster_count() : gridDim.x;
   const uint32_t buf = sm100::smem_addr(dsmem), bar = buf + static_cast<uint32_t>(g.slice) * 16;
   const bool hard = p.labels != nullptr && p.alpha > 0.0f;
-  const Exps<kMode> x{p.cT, kLog2e, g.squarings};
+  const Exps<kMode> x{p.cT, g.squarings};
   const int p0 = static_cast<int>(rank) * g.slice;
   const int C = static_cast<int>(p.C);
 
@@ -631,25 +679,25 @@ __global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kern
     };
     if (list_warp) {
       // The row's list: every CTA of a cluster has all of it, sums the teacher's weights and marks its own columns.
-      float nt = -INFINITY;
+      float mt = -INFINITY;
       auto stage = [&](int k, int id, float t) {
         const int col = id >= 0 && id < C ? id : -1, at = place(col);
         col_s[k] = col, t_s[k] = t;
-        if (col >= 0 && k < p.K) nt = fmaxf(nt, t * p.cT);
+        if (col >= 0 && k < p.K) mt = fmaxf(mt, t);
         if (p.dz && at >= 0 && (atomicOr(bits + (at >> 5), 1u << (at & 31)) & (1u << (at & 31)))) twice = true;
       };
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
         if (lane + 32 * i < entries) stage(lane + 32 * i, ahead_id[i], ahead_t[i]);
       for (int k = lane + 32 * kAhead; k < entries; k += 32) stage(k, list_id(row, k), list_t(row, k));
-      nt = warp_max(nt);
-      if (nt == -INFINITY) nt = 0.0f;
+      RowStats rt;
+      refer_teacher(p, warp_max(mt), rt);
       __syncwarp();
       float st = 0.0f;
       for (int k = lane; k < p.K; k += 32)
-        if (col_s[k] >= 0) st += ex2(fmaf(t_s[k], p.cT, -nt));
+        if (col_s[k] >= 0) st += teacher_weight(rt, t_s[k]);
       st = warp_sum(st);
-      if (lane == 0) teach[par][0] = nt, teach[par][1] = st, teach[par][2] = col_s[p.K] >= 0 ? 1.0f : 0.0f;
+      if (lane == 0) teach[par][0] = rt.ct, teach[par][1] = rt.nt, teach[par][2] = st, teach[par][3] = col_s[p.K] >= 0 ? 1.0f : 0.0f;
     }
     if (pn > 0 && piped) {
       if (!sm100::mbar_wait_bounded(bar, phase, rowk::kRowWaitBudgetNs)) wait_failed = 1;
@@ -662,16 +710,15 @@ __global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kern
 #pragma unroll 4
       for (int pi = tid; pi < pn; pi += nthreads) m = fmaxf(m, max_of(row_s[pi]));
       m = warp_max(m);
-      const float ref = m == -INFINITY ? 0.0f : m;
-      const float n = __fmul_rn(ref, p.cT), n1 = x.n1_of(ref);
+      x.refer(m, r);
       uint64_t s2 = pair(0.0f, 0.0f), s12 = s2;
-      if (warp == 0 && rank == 0) x.add(pair(edge_col >= 0 ? fe : -INFINITY, -INFINITY), n, n1, s2, s12);
+      if (warp == 0 && rank == 0) x.add(pair(edge_col >= 0 ? fe : -INFINITY, -INFINITY), r, s2, s12);
 #pragma unroll 4
       for (int pi = tid; pi < pn; pi += nthreads) {
         uint64_t f[kN / 2];
         unpack_pairs<T>(row_s[pi], f);
 #pragma unroll
-        for (int e = 0; e < kN / 2; ++e) x.add(f[e], n, n1, s2, s12);
+        for (int e = 0; e < kN / 2; ++e) x.add(f[e], r, s2, s12);
       }
       const float2 a = split(s2), b = split(s12);
       const float s = warp_sum(a.x + a.y), s1 = kMode == kOneExp ? 0.0f : warp_sum(b.x + b.y);
@@ -688,9 +735,9 @@ __global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kern
       const bool in = lane < nwarps;
       const float a = in ? red[par][0][lane] : -INFINITY;
       m = warp_max(a);
-      r.S = warp_sum(in ? red[par][1][lane] * (a == m ? 1.0f : ex2(__fmul_rn(a, p.cT) - __fmul_rn(m, p.cT))) : 0.0f);
-      r.S1 = kMode == kOneExp ? r.S : warp_sum(in ? red[par][2][lane] * (a == m ? 1.0f : ex2(x.n1_of(a) - x.n1_of(m))) : 0.0f);
-      r.nt = teach[par][0], r.St = teach[par][1];
+      r.S = warp_sum(in ? red[par][1][lane] * x.weight(a, m, p.cT) : 0.0f);
+      r.S1 = kMode == kOneExp ? r.S : warp_sum(in ? red[par][2][lane] * x.weight1(a, m) : 0.0f);
+      r.ct = teach[par][0], r.nt = teach[par][1], r.St = teach[par][2];
     }
     if (g.ranks > 1) {
       if (warp == 0 && lane < g.ranks) {
@@ -705,8 +752,8 @@ __global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kern
       r.S = r.S1 = 0.0f;
       for (int k = 0; k < g.ranks; ++k) {
         const float pm = peer[par][k][0];
-        r.S += peer[par][k][1] * (pm == a ? 1.0f : ex2(__fmul_rn(pm, p.cT) - __fmul_rn(a, p.cT)));
-        r.S1 += peer[par][k][2] * (pm == a ? 1.0f : ex2(x.n1_of(pm) - x.n1_of(a)));
+        r.S += peer[par][k][1] * x.weight(pm, a, p.cT);
+        r.S1 += peer[par][k][2] * x.weight1(pm, a);
       }
       m = a;
       if constexpr (kMode == kOneExp) r.S1 = r.S;
@@ -715,12 +762,8 @@ __global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kern
         p.loss[owed] = owed_base;
       }
     }
-    {
-      const float ref = m == -INFINITY ? 0.0f : m;
-      r.n = __fmul_rn(ref, p.cT);
-      r.n1 = x.n1_of(ref);
-    }
-    finish_stats<kMode>(p, teach[par][2] != 0.0f, r);
+    x.refer(m, r);
+    finish_stats<kMode>(p, teach[par][3] != 0.0f, r);
     const bool dead = !r.some && !r.known;
     T* out = static_cast<T*>(p.dz) + row * p.lddz;
     if (p.dz && !list_warp) {
@@ -754,12 +797,12 @@ __global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kern
       // this CTA's part of the loss, and the corrections of its columns: equal columns are corrected once, by their first
       // entry, for the sum of their weights in the list's order
       const bool dup = __any_sync(0xffffffffu, twice);
-      auto weight = [&](int j) { return j == p.K ? p.grad_hard : p.grad_soft * target(p, r, t_s[j]); };
+      auto weight = [&](int j) { return j == p.K ? p.grad_hard : p.grad_soft * target(r, t_s[j]); };
       float own = 0.0f;
       for (int k = lane; k < entries; k += 32) {
         const int col = col_s[k], at = place(col);
         if (at < 0) continue;
-        if (k < p.K && r.some) own += cross_term(p, r, t_s[k], z_s[k]);
+        if (k < p.K && r.some) own += cross_term<kMode>(p, r, t_s[k], z_s[k]);
         if (!p.dz) continue;
         bits[at >> 5] = 0u;  // this row's marks go
         float w = 0.0f;
@@ -777,7 +820,7 @@ __global__ void __launch_bounds__(kRowThreads + 32, kRowCtas) distill_block_kern
       }
       own = loss_of_list(p, warp_sum(own));
       if (lane == 0) {
-        if (r.known && place(col_s[p.K]) >= 0) own += loss_of_label(p, r, z_s[p.K], x.c1);
+        if (r.known && place(col_s[p.K]) >= 0) own += loss_of_label<kMode>(p, r, z_s[p.K]);
         if (g.ranks > 1) st_peer_shared(&peer[par][rank][3], 0, own);
         else p.loss[row] = loss_of_sums(p, r) + own;
       }
@@ -951,7 +994,7 @@ bool distill_check(DType dt, const TensorDesc* in, int ni, const TensorDesc* out
     if (!read_attr_payload(attr, schema::kDistill, false, v, 12)) return false;
     p.scale = v[0], p.temperature = v[1], p.alpha = v[2];
   }
-  if (!(p.temperature > 0.0f) || !(p.temperature <= 3.0e38f) || !(p.alpha >= 0.0f) || !(p.alpha <= 1.0f)) return false;
+  if (!(p.temperature >= 0x1p-60f) || !(p.temperature <= 0x1p60f) || !(p.alpha >= 0.0f) || !(p.alpha <= 1.0f)) return false;
   if (ni == 4) {
     const TensorDesc& Y = in[3];
     if (Y.dtype != DType::kI32 || Y.rank() != 1 || !Y.contiguous || Y.shape[0] != p.B) return false;
@@ -959,6 +1002,7 @@ bool distill_check(DType dt, const TensorDesc* in, int ni, const TensorDesc* out
   } else if (p.alpha > 0.0f) {
     return false;  // a label term without labels
   }
+  p.invT = 1.0f / p.temperature;
   p.cT = kLog2e / p.temperature;
   p.grad_soft = p.scale * (1.0f - p.alpha) * p.temperature;
   p.grad_hard = p.scale * p.alpha;

@@ -190,3 +190,49 @@ def test_many_rows_twice_and_replayed(gpu, B, C, K, dtype):
     _C.graph_reset()
     assert np.array_equal(D.float_numpy(), d) and np.array_equal(L.numpy(), l)
     assert _C.wait_status() == 0
+
+
+LOWEST = {"f32": -3.4028235e38, "bf16": -3.3895314e38, "f16": -65504.0}
+
+
+@pytest.mark.parametrize("T,alpha", [(1.0, 0.0), (1.0, 0.5), (2.0, 0.5), (4.0, 0.25), (1.5, 0.5), (0.25, 0.5)])
+@pytest.mark.parametrize("C,K,dtype", [(500, 6, "f32"), (1000, 40, "bf16"), (1000, 8, "f16"), (20000, 12, "bf16"), (40001, 70, "f32")])
+def test_rows_that_a_mask_leaves_nothing_of(gpu, C, K, dtype, T, alpha):
+    """Every logit of a row (its teacher's, too) replaced by a large negative number: the softmax is that of the differences,
+    uniform where the numbers are equal. Differences of equal logits are exact, so no error grows with the logits' size:
+    32 2^-23 relative on sums of C and K equal terms and their quotients, and the types' half steps."""
+    values = [-1e4, LOWEST[dtype]] if dtype == "f16" else [-1e9, -3e9, -1e15, -1e30, LOWEST[dtype], -LOWEST[dtype]]
+    B = 2 * len(values) + 1
+    z, ids, t, y = batch(B, C, K, dtype, seed=C + K)
+    for i, v in enumerate(values):
+        z[2 * i] = z[2 * i + 1] = v
+        t[2 * i] = v
+    z[1, :: C // 7] *= 1.5 if dtype == "f16" else 2.0  # below the others by a whole factor: weighs nothing
+    t[-1] = LOWEST["f32"]
+    z, t = Tensor.from_numpy(z, dtype).float_numpy(), t.astype(np.float32)
+    d, l = run(z, ids, t, y if alpha else None, dtype, 1.0, T, alpha)
+    wd, wl = oracle.distill_ce(z, ids, t, y if alpha else None, 1.0, T, alpha)
+    plain = np.arange(B - 1)  # the last row is an ordinary one with a masked teacher
+    size = np.abs(wd) + (1 - alpha) * T / np.maximum(1, (t == t.max(1, keepdims=True)).sum(1, keepdims=True)) + alpha
+    tiny = 2.0 ** -25 if dtype == "f16" else 1e-37
+    listed = np.zeros((B, C), bool)
+    np.put_along_axis(listed, ids, True, 1)
+    if alpha:
+        listed[np.arange(B), y] = True
+    bound = np.where(listed, size, np.abs(wd)) * 128 * 2.0 ** -23 + np.abs(wd) * EPS_HALF[dtype] * (1 + 2.0 ** -6) + tiny
+    assert np.all(np.abs(d - wd)[plain] <= bound[plain]), f"gradient off by {np.abs(d - wd)[plain].max():.3e}"
+    with np.errstate(over="ignore"):
+        fits = np.abs(wl) < 3e38
+        assert np.all(np.isposinf(l[~fits]))
+        assert np.all(np.abs(l - wl)[fits] <= 128 * 2.0 ** -23 * (np.abs(wl[fits]) + 20 * T * T)), (l, wl)
+    assert np.abs(d[-1] - wd[-1]).max() <= 128 * 2.0 ** -23 * T + EPS_HALF[dtype] * np.abs(wd[-1]).max()
+
+
+@pytest.mark.parametrize("C,K,dtype", [(500, 6, "f32"), (20000, 12, "bf16"), (40001, 70, "f32")])
+def test_a_listed_column_with_the_lowest_logit_has_a_finite_loss(gpu, C, K, dtype):
+    z, ids, t, y = batch(3, C, K, dtype, seed=K)
+    z[0, ids[0, 1]] = z[1, y[1]] = LOWEST[dtype]
+    d, l = run(z, ids, t, y, dtype, 1.0, 1.0, 0.25)
+    wd, wl = oracle.distill_ce(z, ids, t, y, 1.0, 1.0, 0.25)
+    assert np.all(np.abs(l - wl) <= 128 * 2.0 ** -23 * (np.abs(wl) + 20)), (l, wl)
+    assert np.all(np.abs(d - wd) <= 128 * 2.0 ** -23 + EPS_HALF[dtype] * np.abs(wd))
