@@ -127,14 +127,13 @@ __device__ __forceinline__ void values8(const uint32_t (&w)[Mag<T>::kWords], flo
   }
 }
 
-// A p that lies exactly between two values of the format moves one step towards the exact quotient x F / amax. The sign of
-// x F - p amax comes from both products' heads and errors: the heads are equal to a few units, so their difference is exact.
-__device__ __forceinline__ float off_the_tie(float p, float x, float amax, float top) {
-  if (amax > 0x1p90f) x *= 0x1p-40f, amax *= 0x1p-40f;  // both products in range; x is at least 2^-33 of amax here
-  const float have = p * amax, want = x * top;
-  const float d = (want - have) + (fmaf(x, top, -want) - fmaf(p, amax, -have));
-  const float towards = p < 0.0f ? -d : d;  // > 0: the quotient's magnitude is larger
-  const int step = towards > 0.0f ? 1 : towards < 0.0f ? -1 : 0;
+// A p that lies exactly between two values of the format moves one step towards the exact quotient x F / amax, by the sign of
+// x F - p amax: both products are exact in 64 bits (in pairs of fp32 numbers they overflow for blocks above 2^112).
+// Not inlined: its registers would cost every value (8192 x 8192 fp32 tiles: 104 against 78 us).
+__device__ __noinline__ float off_the_tie(float p, float x, float amax, float top) {
+  const double d = fma(static_cast<double>(x), static_cast<double>(top), -static_cast<double>(p) * static_cast<double>(amax));
+  const double towards = p < 0.0f ? -d : d;  // > 0: the quotient's magnitude is larger
+  const int step = towards > 0.0 ? 1 : towards < 0.0 ? -1 : 0;
   return __int_as_float(__float_as_int(p) + step);
 }
 
