@@ -131,7 +131,7 @@ def test_distill_contract():
     assert dce([D((8, 100), "f32", (104, 1)), ids, D((8, 5), "bf16")], [D((8, 100), "f32", (128, 1)), l])
     assert not dce([z, ids, t], [z, l], half), "a label term without labels"
     for bad in ({"scale": 1.0, "temperature": 0.0}, {"scale": 1.0, "temperature": -1.0}, {"scale": 1.0, "temperature": float("nan")},
-                {"scale": 1.0, "temperature": float("inf")}, {"scale": 1.0, "alpha": 1.5}, {"scale": 1.0, "alpha": -0.1}, {"scale": 1.0, "alpha": float("nan")}):
+                {"scale": 1.0, "temperature": float("inf")}, {"scale": 1.0, "temperature": 2.0 ** -61}, {"scale": 1.0, "temperature": 2.0 ** 61}, {"scale": 1.0, "alpha": 1.5}, {"scale": 1.0, "alpha": -0.1}, {"scale": 1.0, "alpha": float("nan")}):
         assert not dce([z, ids, t, y], [z, l], bad), bad
     assert not dce([z, ids, t], [z, l], (0x45434D53, struct.pack("<f", 1.0))), "another op's attributes"
     assert not dce([z, ids, t], [z, l], (0x4C545344, struct.pack("<ff", 1.0, 1.0))), "short payload"
