@@ -13,7 +13,7 @@ scripts print max|delta| against torch), and it has no CPU implementation. So:
     tests/test_ref_parity.py, tests/test_layernorm_gpu.py; and on any machine against the outputs of
     those kernels stored in tests/golden/ref_cuda_golden.npz - tests/test_oracle_cpu.py;
   * softmax, softmax_ce, last-axis sum/max/mean, every bf16 variant, Adam weight decay and the
-    fused-step Adam do not exist in the reference: for those, PARITY IS UNPINNED by the reference and
+    fused-step Adam, quant_fp8, the block-scaled 8-bit products and distill_ce do not exist in the reference: for those, PARITY IS UNPINNED by the reference and
     the fp64 restatement of the published definitions below is the only oracle.
 Structural fixtures the reference does commit (lowered-op list, binding-plan roles, runtime trace
 strings) are checked in tests/test_boundary_fixture.py.
