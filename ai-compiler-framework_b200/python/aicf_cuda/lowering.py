@@ -78,6 +78,8 @@ def build_mlp_train_step(batch: int, dims: Sequence[int], *, compute_dtype: str 
     distill = loss == "distill"
     if distill and not 1 <= teacher_top <= 1024:
         raise ValueError(f"loss='distill' needs 1 <= teacher_top <= 1024, got {teacher_top}")
+    if distill and not (2.0 ** -60 <= temperature <= 2.0 ** 60 and 0.0 <= alpha <= 1.0):
+        raise ValueError(f"loss='distill' needs a temperature in [2^-60, 2^60] and an alpha in [0, 1], got {temperature} and {alpha}")
     if distill and with_argmax:
         raise ValueError("loss='distill' has no arg-max output")
     gb = int(global_batch or batch)

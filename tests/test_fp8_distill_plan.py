@@ -55,7 +55,8 @@ def test_lowering_of_the_distillation_step():
 
 @pytest.mark.parametrize("kw", [dict(linear="int8"), dict(linear="fp8", compute_dtype="f32"), dict(linear="fp8", data_parallel="fused"),
                                 dict(linear="fp8", fp8_grad="f16"), dict(loss="mse"), dict(loss="distill"), dict(loss="distill", teacher_top=2000),
-                                dict(loss="distill", teacher_top=4, with_argmax=True)])
+                                dict(loss="distill", teacher_top=4, with_argmax=True), dict(loss="distill", teacher_top=4, alpha=-0.5),
+                                dict(loss="distill", teacher_top=4, temperature=0.0)])
 def test_lowering_refuses(kw):
     with pytest.raises(ValueError):
         lowered(32, [20, 12], **kw)
