@@ -161,6 +161,10 @@ __global__ void __launch_bounds__(256) distill_multipass_kernel(const DistillPar
 //                          three CTAs per SM in different phases keep loads, exponentials and stores going side by side
 //   distill_multipass_kernel  z and dz misaligned against each other, or a row past eight slices
 //
+// Measured: 65536 x 1000 bf16, T = 2 with labels, 82 us (3.2 TB/s; instruction issue bounds it), f32 without labels 106 us (4.9);
+// 8192 x 32000 f32 in two slices 375 us (5.6 TB/s); 4096 x 100003 bf16, T = 1.5 with labels, 545 us (two exponentials per logit and
+// pass are 365 us by themselves), without labels 377 us (4.3).
+//
 // A row may start anywhere: the whole 16-byte packets inside it are handled as packets, the up to 2 * (kN - 1) elements
 // before and after them one per thread.
 __device__ int g_distill_status = 0;

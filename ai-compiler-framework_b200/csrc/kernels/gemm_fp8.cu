@@ -16,6 +16,10 @@
 // An operand contiguous along M / N instead of K is described to the MMA as MN-major, so no transposed copy is made.
 // Operands that TMA cannot address (rows not 16-byte aligned, or neither stride one) are first copied to aligned rows in
 // the workspace by repitch_kernel.
+//
+// What bounds a long K is the epilogue warps' chain per k block (barrier, tensor-memory load, scale, add): 8192^3 takes 520 us
+// (2.1 PFLOP/s), of which the MMAs alone would need about 340 and the epilogue without any MMA takes 370 to 480. With 1000 along
+// K it is storing the tiles (65536 x 8192: 710 us, with a mask 1310), with one row reading B (8192 x 8192: 23 us as called).
 #include <cstdlib>
 #include <type_traits>
 

@@ -15,7 +15,8 @@
 // A block of threads owns one 128 x 128 tile and keeps it in registers as it was read, eight columns of kRows rows per
 // thread, so all forms come from one read. HBM bounds it (4 bytes per bf16 value for both forms), with instruction issue close
 // behind: about 17 instructions per value for two forms, hence packed 16-bit maxima, one division per row and column of the
-// tile, and the exact rounding below without a branch in the usual case.
+// tile, and the exact rounding below without a branch in the usual case. Measured: 65536 x 8192 bf16, both forms, 485 us (4.5 TB/s),
+// the row form alone 287 us (5.7); 8192 x 8192 f32 tiles 78 us (4.3).
 //
 // Rounding. p = x inv + x inv_lo with inv + inv_lo = F / amax to 2^-48 is x F / amax rounded to fp32. Rounding p to eight bits
 // gives the right value unless p is exactly half way between two of them, where the quotient itself may lie to either side:
